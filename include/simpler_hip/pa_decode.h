@@ -48,8 +48,20 @@ enum { SIMPLER_HIP_DT_FLOAT32 = 0, SIMPLER_HIP_DT_FLOAT16 = 1, SIMPLER_HIP_DT_BF
  * FP16: fp16 query and caches (the dtype of the reference's GQA scene cases,
  * tests/st/a2a3/tensormap_and_ringbuffer/spmd_paged_attention_highperf/
  * test_spmd_paged_attention_highperf.py:170-232); p is rounded to fp16 as
- * the golden rounds it to the input dtype; GQA path (not MLA). */
-enum { SIMPLER_HIP_KV_BF16 = 0, SIMPLER_HIP_KV_FP8_E4M3 = 1, SIMPLER_HIP_KV_FP16 = 2 };
+ * the golden rounds it to the input dtype; GQA path (not MLA).
+ * INT4_BF16, INT4_FP16: bf16 or fp16 query, caches of 4-bit codes in the pages
+ * that include/simpler_hip/kv_cache.h describes, with one fp16 scale and zero
+ * per token, kv head and group of kv_group dims; head dims 64, 128, 256, groups
+ * of 32, 64 or 128 dims (at most 4 per row), block sizes 16/32/64/128, GQA path
+ * (not MLA). p is not rounded before the row sum; p times V's scale is rounded
+ * to fp16 before PV (FLOAT32 out: to 22 bits). No counterpart in the reference. */
+enum {
+    SIMPLER_HIP_KV_BF16 = 0,
+    SIMPLER_HIP_KV_FP8_E4M3 = 1,
+    SIMPLER_HIP_KV_FP16 = 2,
+    SIMPLER_HIP_KV_INT4_BF16 = 3,
+    SIMPLER_HIP_KV_INT4_FP16 = 4
+};
 
 /*
  * One paged-attention decode call. All pointers are device pointers.
@@ -63,10 +75,14 @@ enum { SIMPLER_HIP_KV_BF16 = 0, SIMPLER_HIP_KV_FP8_E4M3 = 1, SIMPLER_HIP_KV_FP16
  * value_cache  same element type, same addressing with the v_* strides and Dv columns.
  *              MLA: value_cache == key_cache with the K strides and Dv <= Dk
  *              (V is the first Dv columns of K).
+ *              INT4: uint8 pages, that of (blk, kvh) at blk*block_stride +
+ *              kvh*head_stride bytes, block_size*Dk/2 bytes each;
+ *              *_token_stride is Dk/2 (the pages' own order is fixed).
  * block_table  int32 [batch, max_blocks_per_seq], entries in [0, num_blocks)
  * context_lens int32 [batch], 0 <= len <= max_blocks_per_seq*block_size
  * out          [batch, q_len, num_heads, Dv] of out_dtype: FLOAT32 or BFLOAT16
- *              (bf16 and fp8 caches), FLOAT32 or FLOAT16 (fp16 caches)
+ *              (bf16 and fp8 caches), FLOAT32 or FLOAT16 (fp16 caches); INT4:
+ *              FLOAT32 or the query's type
  * scale        softmax scale applied to q.k in fp32
  * causal       q_len > 1 only: query token i sees context_len - (q_len-1-i) tokens
  */
@@ -95,13 +111,17 @@ typedef struct SimplerHipPaDecodeArgs {
      * number of workers the (tile, KV block) work list is divided among (and
      * keeps short contexts on the work list). */
     int32_t num_workers;
-    /* SIMPLER_HIP_KV_BF16 (0), SIMPLER_HIP_KV_FP8_E4M3 (1) or SIMPLER_HIP_KV_FP16 (2). */
-    int32_t kv_format;
-    /* kv_format FP8_E4M3 only: fp32 [num_blocks, num_kv_heads] dequantisation
-     * scales; cache element (blk, t, kvh, d) stands for
-     * fp8_e4m3fn(byte) * scale[blk * num_kv_heads + kvh]. NULL otherwise. */
-    const float *k_scale;
-    const float *v_scale;
+    int32_t kv_format; /* one of SIMPLER_HIP_KV_* */
+    /* FP8_E4M3: fp32 [num_blocks, num_kv_heads] dequantisation scales; cache
+     * element (blk, t, kvh, d) stands for
+     * fp8_e4m3fn(byte) * scale[blk * num_kv_heads + kvh].
+     * INT4: fp16 [num_blocks, num_kv_heads, Dk / kv_group, block_size, 2], the
+     * scale s and zero z of a token's group: a code c stands for c s + z.
+     * NULL otherwise. */
+    const void *k_scale;
+    const void *v_scale;
+    int32_t kv_group; /* INT4: dims per scale (else not read) */
+    int32_t reserved;
 } SimplerHipPaDecodeArgs;
 
 /* Bytes of device workspace simpler_hip_pa_decode needs for these args
@@ -181,11 +201,13 @@ int simpler_hip_pa_decode_noalloc(const SimplerHipPaDecodeArgs *args, void *stre
  * block_table[b][p / block_size] -- the slot the reference derives from the
  * block table and seq_len (qwen3_14b_decode.py:106-115). Results and cache
  * contents are those of simpler_hip_kv_append with that slot mapping followed
- * by simpler_hip_pa_decode. q_len <= 16; bf16 and fp16 caches (not fp8).
+ * by simpler_hip_pa_decode. q_len <= 16; bf16 and fp16 caches, and 4-bit ones
+ * (key_new and value_new of the query's type, appended as by
+ * simpler_hip_kv4_append); not fp8.
  * The append is fused into the decode's two launches where each worker runs
  * one row tile; where the decode gives a worker several row tiles (GQA with
- * more than 16 query rows per kv head), for MLA and ahead of the one-kernel
- * decode of short contexts, it runs as a launch of its own, which measured
+ * more than 16 query rows per kv head), for MLA, for 4-bit caches and ahead of
+ * the one-kernel decode of short contexts, it runs as a launch of its own, which measured
  * faster there. Both forms leave the same cache contents.
  * Same workspace as simpler_hip_pa_decode for these args. A length below
  * q_len or above max_blocks_per_seq*block_size is reported by

@@ -58,6 +58,8 @@ class PaDecodeArgs(ctypes.Structure):
         ("kv_format", ctypes.c_int32),
         ("k_scale", ctypes.c_void_p),
         ("v_scale", ctypes.c_void_p),
+        ("kv_group", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
     ]
 
 
@@ -105,6 +107,58 @@ class DecodePreludeArgs(ctypes.Structure):
     ]
 
 
+class Kv4Args(ctypes.Structure):
+    """Mirror of ``SimplerHipKv4Args`` (include/simpler_hip/kv_cache.h)."""
+
+    _fields_ = [
+        *[(n, ctypes.c_void_p) for n in ("key", "value", "slot_mapping", "key_cache", "value_cache", "k_scale", "v_scale",
+                                          "error_count")],
+        *[(n, ctypes.c_int64) for n in ("key_token_stride", "key_head_stride", "value_token_stride",
+                                         "value_head_stride", "k_block_stride", "k_head_stride", "v_block_stride",
+                                         "v_head_stride")],
+        *[(n, ctypes.c_int32) for n in ("num_tokens", "num_kv_heads", "head_dim", "block_size", "num_blocks",
+                                         "kv_group", "dtype", "reserved")],
+    ]
+
+
+class QkNormMropeArgs(ctypes.Structure):
+    """Mirror of ``SimplerHipQkNormMropeArgs`` (include/simpler_hip/kv_cache.h)."""
+
+    _fields_ = [
+        *[(n, ctypes.c_void_p) for n in ("q_proj", "k_proj", "v_proj", "inv_rms", "q_norm_weight", "k_norm_weight",
+                                          "rope_cos", "rope_sin", "positions", "slot_mapping", "q_out", "key_cache",
+                                          "value_cache", "error_count")],
+        *[(n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride", "k_block_stride", "k_token_stride",
+                                         "k_head_stride", "v_block_stride", "v_token_stride", "v_head_stride")],
+        *[(n, ctypes.c_int32) for n in ("num_tokens", "num_heads", "num_kv_heads", "head_dim", "block_size",
+                                         "num_blocks", "max_position", "proj_dtype", "dtype", "num_axes",
+                                         "interleaved")],
+        ("sections", ctypes.c_int32 * 4),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class ReleaseBlocksArgs(ctypes.Structure):
+    """Mirror of ``SimplerHipReleaseBlocksArgs`` (include/simpler_hip/step_plan.h)."""
+
+    _fields_ = [
+        *[(n, ctypes.c_void_p) for n in ("ended", "context_lens", "block_table", "free_blocks", "free_count",
+                                          "context_lens_out", "free_count_out", "error_count")],
+        *[(n, ctypes.c_int32) for n in ("batch", "max_blocks_per_seq", "block_size", "capacity")],
+    ]
+
+
+class AssignSlotsArgs(ctypes.Structure):
+    """Mirror of ``SimplerHipAssignSlotsArgs`` (include/simpler_hip/step_plan.h)."""
+
+    _fields_ = [
+        *[(n, ctypes.c_void_p) for n in ("new_lens", "context_lens", "block_table", "free_blocks", "free_count",
+                                          "slot_mapping", "positions", "requests", "starts", "context_lens_out",
+                                          "granted", "free_count_out", "error_count")],
+        *[(n, ctypes.c_int32) for n in ("batch", "max_blocks_per_seq", "block_size", "capacity", "num_tokens")],
+    ]
+
+
 # Every symbol the public headers declare, with its ctypes signature.
 _VP, _SZ, _I32, _U32, _U64, _I = (
     ctypes.c_void_p,
@@ -131,6 +185,12 @@ SIGNATURES: dict[str, tuple] = {
     # include/simpler_hip/kv_cache.h
     "simpler_hip_kv_append": (_I, [ctypes.POINTER(KvAppendArgs), _VP]),
     "simpler_hip_qk_norm_rope_append": (_I, [ctypes.POINTER(QkNormRopeAppendArgs), _VP]),
+    "simpler_hip_kv4_append": (_I, [ctypes.POINTER(Kv4Args), _VP]),
+    "simpler_hip_kv4_gather": (_I, [ctypes.POINTER(Kv4Args), _VP]),
+    "simpler_hip_qk_norm_mrope_append": (_I, [ctypes.POINTER(QkNormMropeArgs), _VP]),
+    # include/simpler_hip/step_plan.h
+    "simpler_hip_release_blocks": (_I, [ctypes.POINTER(ReleaseBlocksArgs), _VP]),
+    "simpler_hip_assign_slots": (_I, [ctypes.POINTER(AssignSlotsArgs), _VP]),
     # include/simpler_hip/pto_runtime_c_api.h
     "get_pipeline_contract": (_VP, []),
     "get_runtime_size": (_SZ, []),

@@ -29,9 +29,15 @@ SOURCES = [
     CSRC / "pa_kernels_direct_bf16.hip",
     CSRC / "pa_kernels_direct_f16.hip",
     CSRC / "pa_kernels_direct_fp8.hip",
+    CSRC / "pa_kernels_int4_d64.hip",
+    CSRC / "pa_kernels_int4_d128.hip",
+    CSRC / "pa_kernels_int4_d256.hip",
     CSRC / "pa_kernels_mla.hip",
     CSRC / "pa_kernels_merge.hip",
     CSRC / "kv_cache.hip",
+    CSRC / "kv_cache4.hip",
+    CSRC / "kv_rotary.hip",
+    CSRC / "step_plan.hip",
     CSRC / "incore_kernels.hip",
     CSRC / "task_graph.cpp",
     CSRC / "orchestrations.cpp",

@@ -33,6 +33,7 @@
 #include <stdint.h>
 
 #include "simpler_hip/kv_cache.h"
+#include "kv_slots.h"
 #include "pa_decode_internal.h"
 
 namespace simpler_hip_kv {
@@ -42,15 +43,6 @@ typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kMaxHeadDim = 1024;
-
-// The paged form's token -> (position, slot) inputs; block_table null: the
-// caller's slot mapping (and seq_lens) instead.
-struct Paged {
-    const int32_t *block_table, *context_lens;
-    unsigned *error_flag;  // the decode workspace's error word
-    unsigned bad_length;   // its bit for a length below q_len (or a position outside the RoPE table)
-    int32_t q_len, max_blocks;
-};
 
 struct AppendParams {
     const uint16_t *key, *value;
@@ -62,30 +54,6 @@ struct AppendParams {
     int32_t num_tokens, hkv, dk, dv, block_size, num_blocks;
     Paged pg;
 };
-
-__device__ __forceinline__ bool slot_ok(int slot, int32_t num_blocks, int32_t block_size, int32_t *err) {
-    if (slot < 0) return false;  // padding token
-    if ((int64_t)slot >= (int64_t)num_blocks * block_size) {
-        if (threadIdx.x == 0 && err) atomicAdd(err, 1);
-        return false;
-    }
-    return true;
-}
-
-// Paged form: position and slot of launch token t, or slot -1 where the
-// token is not written: a position below 0 (a length below q_len, reported
-// by the caller of this), one past the block-table row (a length the decode
-// reports), or an out-of-pool block (reported when the decode reads it).
-__device__ __forceinline__ int paged_slot(const Paged &G, const int t, const int32_t block_size,
-                                          const int32_t num_blocks, int *pos) {
-    const int b = t / G.q_len;
-    const int p = G.context_lens[b] - G.q_len + (t - b * G.q_len);
-    *pos = p;
-    if (p < 0 || p >= G.max_blocks * block_size) return -1;
-    const int phys = G.block_table[(int64_t)b * G.max_blocks + p / block_size];
-    if ((unsigned)phys >= (unsigned)num_blocks) return -1;
-    return phys * block_size + p % block_size;
-}
 
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendParams P) {
     const int t = blockIdx.x;
@@ -241,17 +209,6 @@ void launch_prelude_kernel(const PreludeParams &P, unsigned units, unsigned toke
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
-
-Paged paged_of(const SimplerHipPaDecodeArgs *a, unsigned *error_flag, unsigned bad_length) {
-    Paged G{};
-    G.block_table = a->block_table;
-    G.context_lens = a->context_lens;
-    G.error_flag = error_flag;
-    G.bad_length = bad_length;
-    G.q_len = a->q_len;
-    G.max_blocks = a->max_blocks_per_seq;
-    return G;
-}
 
 }  // namespace
 }  // namespace simpler_hip_kv

@@ -30,6 +30,7 @@ using namespace pa;
 constexpr int kZeroOffset = 128;  // workspace bytes [128, 256) are never written after init
 constexpr int kMaxAppendTokens = 16;  // fused append: new tokens per sequence (one per residue mod 16)
 constexpr size_t kMaxZeroPageBytes = 1 << 20;  // larger token strides read the padding tiles as they are
+constexpr int kInt4WavesPerCu = 8;  // 4-bit caches: worker waves per CU
 constexpr int kMlaSegTokens = 256;  // MLA: work charged for each sequence a slice starts, in tokens
 
 struct Plan {
@@ -51,6 +52,10 @@ struct Plan {
 
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
+inline bool is_int4(const SimplerHipPaDecodeArgs *a) {
+    return a->kv_format == SIMPLER_HIP_KV_INT4_BF16 || a->kv_format == SIMPLER_HIP_KV_INT4_FP16;
+}
+
 int validate(const SimplerHipPaDecodeArgs *a) {
     if (!a) return SIMPLER_HIP_ERR_INVALID;
     if (!a->query || !a->key_cache || !a->value_cache || !a->block_table || !a->context_lens || !a->out)
@@ -62,13 +67,25 @@ int validate(const SimplerHipPaDecodeArgs *a) {
     if (a->block_size < 1 || a->max_blocks_per_seq < 1 || a->num_blocks < 1) return SIMPLER_HIP_ERR_INVALID;
     const int64_t strides[6] = {a->k_block_stride, a->k_token_stride, a->k_head_stride,
                                 a->v_block_stride, a->v_token_stride, a->v_head_stride};
-    if (a->kv_format != SIMPLER_HIP_KV_BF16 && a->kv_format != SIMPLER_HIP_KV_FP8_E4M3 &&
-        a->kv_format != SIMPLER_HIP_KV_FP16)
-        return SIMPLER_HIP_ERR_INVALID;
-    const bool fp8 = a->kv_format == SIMPLER_HIP_KV_FP8_E4M3;
-    const int esz = fp8 ? 1 : 2;
+    if (a->kv_format < SIMPLER_HIP_KV_BF16 || a->kv_format > SIMPLER_HIP_KV_INT4_FP16) return SIMPLER_HIP_ERR_INVALID;
+    const bool fp8 = a->kv_format == SIMPLER_HIP_KV_FP8_E4M3, int4 = is_int4(a);
+    const int esz = fp8 || int4 ? 1 : 2;
     for (int64_t s : strides)
         if (s <= 0 || (s * esz) % 16) return SIMPLER_HIP_ERR_INVALID;  // 16-byte aligned rows
+    if (int4) {
+        if (a->kv_group < 1 || a->head_dim_k != a->head_dim_v || a->head_dim_k % a->kv_group)
+            return SIMPLER_HIP_ERR_INVALID;
+        if (a->k_token_stride != a->head_dim_k / 2 || a->v_token_stride != a->head_dim_k / 2)
+            return SIMPLER_HIP_ERR_INVALID;  // a page's rows
+        if (!a->k_scale || !a->v_scale || ((uintptr_t)a->k_scale & 3) || ((uintptr_t)a->v_scale & 3))
+            return SIMPLER_HIP_ERR_INVALID;
+        if (a->block_size != 16 && a->block_size != 32 && a->block_size != 64 && a->block_size != 128)
+            return SIMPLER_HIP_ERR_UNSUPPORTED;
+        // positions within a sequence are 32-bit
+        if ((int64_t)a->max_blocks_per_seq * a->block_size >= (int64_t)1 << 31) return SIMPLER_HIP_ERR_UNSUPPORTED;
+        const int half = a->kv_format == SIMPLER_HIP_KV_INT4_FP16 ? SIMPLER_HIP_DT_FLOAT16 : SIMPLER_HIP_DT_BFLOAT16;
+        if (a->out_dtype != SIMPLER_HIP_DT_FLOAT32 && a->out_dtype != half) return SIMPLER_HIP_ERR_UNSUPPORTED;
+    }
     if (a->k_token_stride * esz * a->block_size >= (int64_t)1 << 31 ||
         a->v_token_stride * esz * a->block_size >= (int64_t)1 << 31)
         return SIMPLER_HIP_ERR_INVALID;  // per-lane 32-bit byte offsets within a block
@@ -108,6 +125,16 @@ struct Kernels {
     MergeFn merge;
 };
 
+KernelPair pick_int4(int d, int groups, int out) {
+    return d == 64 ? pick_int4_d64(groups, out) : d == 128 ? pick_int4_d128(groups, out)
+         : d == 256 ? pick_int4_d256(groups, out) : KernelPair{};
+}
+
+DirectFn pick_int4_direct(int d, int groups, int out) {
+    return d == 64 ? pick_int4_direct_d64(groups, out) : d == 128 ? pick_int4_direct_d128(groups, out)
+         : d == 256 ? pick_int4_direct_d256(groups, out) : DirectFn{};
+}
+
 Kernels pick_kernel(const SimplerHipPaDecodeArgs *a, bool append = false) {
     Kernels s{};
     const int bs = a->block_size, dk = a->head_dim_k, dv = a->head_dim_v, out = a->out_dtype;
@@ -116,6 +143,11 @@ Kernels pick_kernel(const SimplerHipPaDecodeArgs *a, bool append = false) {
         if (dk == dv && !append) {  // no fused append for fp8 caches
             s.k = pick_gqa_fp8(bs, dk, out);
             s.direct = pick_direct_fp8(bs, dk, out);
+        }
+    } else if (is_int4(a)) {
+        if (!append && (a->kv_group == 32 || a->kv_group == 64 || a->kv_group == 128)) {  // no fused append
+            s.k = pick_int4(dk, dk / a->kv_group, out);
+            s.direct = pick_int4_direct(dk, dk / a->kv_group, out);
         }
     } else if (is_mla_shape(a)) {
         // (the kernel's fill offsets use 24-bit multiplies: token rows below 8 MB)
@@ -219,6 +251,7 @@ int wave_slots(KernelFn fn, int threads, int want_per_cu, size_t lds = 0) {
 // A plan made without a device (which can launch nothing) reports `nominal`
 // counts that do not depend on the block size.
 int workers_per_cu(const SimplerHipPaDecodeArgs *a, const KernelPair &k, const Plan &p, bool pair, bool nominal) {
+    if (is_int4(a)) return kInt4WavesPerCu;
     if (pair) return kWorkersThreePerCu;
     const int bs = a->block_size, d = a->head_dim_k, tiles = p.tiles_per_worker;
     const bool fp8 = a->kv_format == SIMPLER_HIP_KV_FP8_E4M3;
@@ -275,8 +308,10 @@ Plan make_plan(const SimplerHipPaDecodeArgs *a, const KernelPair &k) {  // k: th
         // Row tiles of one kv head run as sibling waves of one worker workgroup
         // (up to four), so K/V of a block is fetched once for all of them;
         // two row tiles with K through LDS run in one wave instead.
-        const bool pair = k.main_pair && p.row_tiles == 2;
-        p.tiles_per_worker = pair ? 2 : (p.row_tiles < kMaxWavesPerWorker ? p.row_tiles : kMaxWavesPerWorker);
+        // 4-bit caches: pairs of row tiles, without siblings.
+        const bool int4 = is_int4(a);
+        const bool pair = k.main_pair && (int4 ? p.row_tiles >= 2 : p.row_tiles == 2);
+        p.tiles_per_worker = pair ? 2 : int4 ? 1 : (p.row_tiles < kMaxWavesPerWorker ? p.row_tiles : kMaxWavesPerWorker);
         p.threads = pair ? 64 : 64 * p.tiles_per_worker;
         p.main = pair ? k.main_pair : p.tiles_per_worker > 1 ? k.main_multi : k.main;
         if (!pair && k.klds && p.tiles_per_worker > 1) p.lds = (size_t)p.tiles_per_worker * a->block_size * 256;
@@ -315,7 +350,7 @@ Plan make_plan(const SimplerHipPaDecodeArgs *a, const KernelPair &k) {  // k: th
     const int esz = a->kv_format == SIMPLER_HIP_KV_FP8_E4M3 ? 1 : 2;
     const size_t tok_bytes = (size_t)std::max(a->k_token_stride, a->v_token_stride) * esz;
     const size_t zero_bytes = align_up(16 * tok_bytes + 512, 256);
-    p.zero_bytes = (!k.mla && zero_bytes <= kMaxZeroPageBytes) ? zero_bytes : 0;
+    p.zero_bytes = (!k.mla && !is_int4(a) && zero_bytes <= kMaxZeroPageBytes) ? zero_bytes : 0;
     const size_t pieces = (size_t)p.workers * p.tiles_per_worker * 2;
     p.flag_bytes = 256;  // error word at 0, zeros at [kZeroOffset, 256)
     p.part_ml_bytes = align_up(pieces * 32 * sizeof(float), 256);
@@ -356,8 +391,17 @@ Plan make_plan(const SimplerHipPaDecodeArgs *a, const KernelPair &k) {  // k: th
 //   174 / 127; 15 x 8 of 380 tokens, 64 rows of 128 dims, 90 MB, 23.5 / 20.9).
 //   Above 64 dims, 768 KB over the row tiles of a kv head at most.
 // Waves per tile: enough for workers_per_cu waves on every CU, at least four.
+int int4_direct_waves(const SimplerHipPaDecodeArgs *a, const Kernels &s, const Plan &p) {
+    const int64_t tokens = (int64_t)a->max_blocks_per_seq * a->block_size;
+    const int64_t chunks = (tokens + 63) / 64;
+    const int64_t waves = std::min<int64_t>(s.direct.max_waves, chunks);
+    if ((chunks + waves - 1) / waves > 2) return 0;
+    return (int)waves;
+}
+
 int direct_waves(const SimplerHipPaDecodeArgs *a, const Kernels &s, const Plan &p) {
     if (!s.direct.fn || a->num_workers > 0) return 0;
+    if (is_int4(a)) return int4_direct_waves(a, s, p);
     const int bs = a->block_size, d = a->head_dim_k;
     const bool fp8 = a->kv_format == SIMPLER_HIP_KV_FP8_E4M3, narrow = fp8 || d <= 64;
     const int64_t blocks = a->max_blocks_per_seq, block = (int64_t)bs * 2 * d * (fp8 ? 1 : 2);
@@ -525,7 +569,9 @@ extern "C" const char *simpler_hip_pa_decode_kernel_name(const SimplerHipPaDecod
     const Kernels s = pick_kernel(args);
     if (!s.k.main) return "";
     if (s.k.mla) return "pa_mla_kernel";
-    return pick_route(args, s, make_plan(args, s.k)).waves ? "pa_direct_kernel" : "pa_decode_kernel";
+    const bool direct = pick_route(args, s, make_plan(args, s.k)).waves != 0;
+    if (is_int4(args)) return direct ? "pa_int4_direct_kernel" : "pa_int4_kernel";
+    return direct ? "pa_direct_kernel" : "pa_decode_kernel";
 }
 
 extern "C" int simpler_hip_pa_decode(const SimplerHipPaDecodeArgs *a, void *workspace, size_t workspace_bytes,
@@ -587,8 +633,9 @@ int pa_decode_launch(const SimplerHipPaDecodeArgs *a, void *workspace, size_t wo
     P.seg_cost = plan.seg_cost;
     P.scale = a->scale;
     P.causal = (a->causal && a->q_len > 1) ? 1 : 0;
-    P.k_scale = a->k_scale;
-    P.v_scale = a->v_scale;
+    P.k_scale = (const float *)a->k_scale;
+    P.v_scale = (const float *)a->v_scale;
+    P.half16 = a->kv_format == SIMPLER_HIP_KV_INT4_FP16;
     P.err_mirror = (phases & SIMPLER_HIP_PHASE_MERGE) ? err_mirror : nullptr;
     P.k_new = (const uint16_t *)k_new;
     P.v_new = (const uint16_t *)v_new;
@@ -665,12 +712,12 @@ extern "C" int simpler_hip_pa_decode_append(const SimplerHipPaDecodeArgs *a, con
         const Kernels s = pick_kernel(a);
         if (s.k.main) {
             const Plan plan = make_plan(a, s.k);
-            if (plan.tiles_per_worker > 1 || s.k.mla || pick_route(a, s, plan).waves) {
+            if (plan.tiles_per_worker > 1 || s.k.mla || is_int4(a) || pick_route(a, s, plan).waves) {
                 if (!workspace || workspace_bytes < plan.total || ((uintptr_t)workspace & 255))
                     return SIMPLER_HIP_ERR_WORKSPACE;
                 if (a->batch == 0) return SIMPLER_HIP_OK;
-                const int rc2 =
-                    launch_paged_append(a, key_new, value_new, (unsigned *)workspace, kErrBadLength, stream);
+                const auto append = is_int4(a) ? launch_paged_append4 : launch_paged_append;
+                const int rc2 = append(a, key_new, value_new, (unsigned *)workspace, kErrBadLength, stream);
                 if (rc2 != SIMPLER_HIP_OK) return rc2;
                 return pa_decode_launch(a, workspace, workspace_bytes, stream,
                                         SIMPLER_HIP_PHASE_MAIN | SIMPLER_HIP_PHASE_MERGE, nullptr);

@@ -29,6 +29,10 @@ int pa_decode_with_mirror(const SimplerHipPaDecodeArgs *a, void *workspace, size
 int launch_paged_append(const SimplerHipPaDecodeArgs *a, const void *key_new, const void *value_new,
                         unsigned *error_flag, unsigned bad_length, void *stream);
 
+// The same into 4-bit caches (kv_cache4.hip).
+int launch_paged_append4(const SimplerHipPaDecodeArgs *a, const void *key_new, const void *value_new,
+                         unsigned *error_flag, unsigned bad_length, void *stream);
+
 // The decode prelude (kv_cache.hip) over the same tokens: the bf16 query rows
 // into q_out ([batch, q_len, num_heads, head_dim]) and the new K/V rows into
 // the caches, as simpler_hip_qk_norm_rope_append computes them; a position

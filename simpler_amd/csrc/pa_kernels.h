@@ -132,6 +132,7 @@ struct KernelParams {
     const uint16_t *v_new;
     int32_t merge_units;  // merge kernel: 16-byte units of a tile per workgroup
     int32_t whole_tiles;  // MLA: a workgroup per tile and row group, no work list, no merge
+    int32_t half16;       // 4-bit caches: the query (and a 16-bit output) is fp16, else bf16
 };
 
 __device__ __forceinline__ u32x4_t ld16(const uint16_t *p) { return *reinterpret_cast<const u32x4_t *>(p); }
@@ -2678,6 +2679,15 @@ KernelPair pick_gqa_fp8(int bs, int d, int out_dtype);
 DirectFn pick_direct_bf16(int bs, int d, int out_dtype);
 DirectFn pick_direct_f16(int bs, int d, int out_dtype);
 DirectFn pick_direct_fp8(int bs, int d, int out_dtype);
+// GQA decode with 4-bit caches (pa_kernels_int4.h), Dk == Dv, `groups`
+// scales per row, bf16 or fp16 query: main and main_pair run one and two row
+// tiles per wave.
+KernelPair pick_int4_d64(int groups, int out_dtype);
+KernelPair pick_int4_d128(int groups, int out_dtype);
+KernelPair pick_int4_d256(int groups, int out_dtype);
+DirectFn pick_int4_direct_d64(int groups, int out_dtype);
+DirectFn pick_int4_direct_d128(int groups, int out_dtype);
+DirectFn pick_int4_direct_d256(int groups, int out_dtype);
 // MLA (Dk 576, Dv 512, V a prefix of K), bf16.
 KernelPair pick_mla(int bs, int out_dtype);
 // The split merge for output width dv.

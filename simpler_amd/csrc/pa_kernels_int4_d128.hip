@@ -1,0 +1,26 @@
+// GQA decode with 4-bit caches, head dim 128: every group size it takes.
+#include "pa_kernels_int4.h"
+
+namespace simpler_hip {
+namespace pa {
+
+KernelPair pick_int4_d128(int groups, int out_dtype) {
+    switch (groups) {
+        case 1: return int4_pair<128, 1>(out_dtype);
+        case 2: return int4_pair<128, 2>(out_dtype);
+        case 4: return int4_pair<128, 4>(out_dtype);
+        default: return KernelPair{};
+    }
+}
+
+DirectFn pick_int4_direct_d128(int groups, int out_dtype) {
+    switch (groups) {
+        case 1: return int4_direct<128, 1>(out_dtype);
+        case 2: return int4_direct<128, 2>(out_dtype);
+        case 4: return int4_direct<128, 4>(out_dtype);
+        default: return DirectFn{};
+    }
+}
+
+}  // namespace pa
+}  // namespace simpler_hip

@@ -8,17 +8,25 @@ weight, half-split RoPE at position ``seq_len − 1``, bf16 rounding
 (``:207-226``) — runs fused with that write. Both are kernels in
 ``libsimpler_hip.so`` (``include/simpler_hip/kv_cache.h``); torch supplies device
 memory and the stream only, and there is no fallback.
+
+Around them, also kernels of the library: caches of 4 bits per value
+(``alloc_kv4_pools``, ``kv4_append``, ``kv4_gather``; attended to by
+``paged_attention.paged_attention_decode``), the prelude with rotary positions
+of several axes (``qk_norm_mrope_append``), and a step's block tables and slot
+maps built on the device from the requests' lengths (``release_blocks``,
+``assign_slots``; ``include/simpler_hip/step_plan.h``).
 """
 
 from __future__ import annotations
 
 import ctypes
 import struct
+from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from .paged_attention import PagedAttentionError, _current_stream
+from .paged_attention import _OUT_DTYPES, PagedAttentionError, _current_stream
 
 EPS = 1e-6  # the golden's eps (qwen3_14b_decode.py:46)
 
@@ -258,3 +266,361 @@ def prelude_args(q_proj: torch.Tensor, k_proj: torch.Tensor, v_proj: torch.Tenso
         _dev(error_count, "error_count", torch.int32)
         a.error_count = error_count.data_ptr()
     return a
+
+
+def _launch(name: str, args: ctypes.Structure, device: torch.device, stream: int | None) -> None:
+    """Run the C entry ``name`` on ``stream`` (default: torch's current one of ``device``), with that device current."""
+    fn = getattr(_lib.lib(), name)
+    if stream is None:
+        stream = _current_stream(device)
+    if device.index is None or device.index == torch.cuda.current_device():
+        rc = fn(ctypes.byref(args), stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(ctypes.byref(args), stream)
+    if rc != 0:
+        raise PagedAttentionError(rc, name)
+
+
+# ---------------------------------------------------------------------------
+# Caches of 4 bits per value
+# ---------------------------------------------------------------------------
+
+
+class Kv4Pools(NamedTuple):
+    """4-bit K and V pages and their scales, in the order in which ``kv4_append`` and the decode take them."""
+
+    key_cache: torch.Tensor  # uint8 [num_blocks, kv_heads, block_size, head_dim / 2]
+    value_cache: torch.Tensor
+    k_scale: torch.Tensor  # fp16 [num_blocks, kv_heads, head_dim / group_size, block_size, 2]: scale, zero
+    v_scale: torch.Tensor
+
+
+def alloc_kv4_pools(num_blocks: int, block_size: int, kv_heads: int, head_dim: int, group_size: int = 64,
+                    device: torch.device | str = "cuda") -> Kv4Pools:
+    """Pools for a cache of 4 bits per value, uninitialised.
+
+    A value is held as a 4-bit code c with a scale s and a zero z, both fp16,
+    per token, kv head and group of ``group_size`` dims, and stands for
+    ``c * s + z``: ``head_dim / 2 + 4 * head_dim / group_size`` bytes per row.
+    The order of the codes within a page is the decode kernel's own
+    (``include/simpler_hip/kv_cache.h``): write rows with ``kv4_append``, read them
+    with ``kv4_gather``, and move whole pages (``[block]``) as they are.
+    head_dim 64, 128 or 256; group_size 32, 64 or 128, at most four groups per
+    row; block_size 16, 32, 64 or 128.
+    """
+    if head_dim not in (64, 128, 256) or group_size not in (32, 64, 128) or not group_size <= head_dim <= 4 * group_size:
+        raise ValueError(f"4-bit caches: head_dim 64, 128 or 256 in one, two or four groups of 32, 64 or 128, "
+                         f"got {head_dim} and {group_size}")
+    if block_size not in (16, 32, 64, 128):
+        raise ValueError(f"4-bit caches: block_size 16, 32, 64 or 128, got {block_size}")
+    pages = (num_blocks, kv_heads, block_size, head_dim // 2)
+    scales = (num_blocks, kv_heads, head_dim // group_size, block_size, 2)
+    return Kv4Pools(torch.empty(pages, dtype=torch.uint8, device=device),
+                    torch.empty(pages, dtype=torch.uint8, device=device),
+                    torch.empty(scales, dtype=torch.float16, device=device),
+                    torch.empty(scales, dtype=torch.float16, device=device))
+
+
+def _one_device(first: torch.Tensor, *others: torch.Tensor) -> bool:
+    at = first.get_device()
+    for t in others:
+        if t.get_device() != at:
+            return False
+    return True
+
+
+# SimplerHipKv4Args as _lib.Kv4Args lays it out
+_KV4 = struct.Struct("@8P8q8i")
+assert _KV4.size == ctypes.sizeof(_lib.Kv4Args)
+
+
+def _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, dtypes) -> _lib.Kv4Args:
+    """Check the tensors of a 4-bit append or gather (rows of one of ``dtypes``) and fill the C args."""
+    rt = key.dtype
+    tokens, hkv, dim = key.shape
+    nblk, chkv, bs, row = key_cache.shape
+    kt, kh, k1 = key.stride()
+    vt, vh, v1 = value.stride()
+    kb, kch, kcr, kc1 = key_cache.stride()
+    vb, vch, vcr, vc1 = value_cache.stride()
+    groups = k_scale.shape[2]
+    if tokens <= 1:  # strides of dims of one element say nothing
+        kt = vt = 8
+    if hkv == 1:
+        kh = vh = 8
+        kch = vch = 16
+    if nblk == 1:
+        kb = vb = 16
+    err = 0 if error_count is None else error_count.data_ptr()
+    u8, f16, i32 = torch.uint8, torch.float16, torch.int32
+    if not (
+        rt in dtypes and value.dtype is rt and value.shape == key.shape and k1 == 1 and v1 == 1
+        and key_cache.dtype is u8 and value_cache.dtype is u8 and value_cache.shape == key_cache.shape
+        and chkv == hkv and 2 * row == dim and kcr == row and kc1 == 1 and vcr == row and vc1 == 1
+        and k_scale.dtype is f16 and v_scale.dtype is f16 and k_scale.shape == (nblk, hkv, groups, bs, 2)
+        and v_scale.shape == k_scale.shape and k_scale.is_contiguous() and v_scale.is_contiguous()
+        and groups > 0 and dim % groups == 0 and slot_mapping.dtype is i32 and slot_mapping.shape == (tokens,)
+        and slot_mapping.is_contiguous() and key.is_cuda
+        and (error_count is None or (error_count.dtype is i32 and error_count.is_cuda))
+        and _one_device(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale)
+    ):
+        _refuse_kv4(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, dtypes)
+    return _lib.Kv4Args.from_buffer_copy(_KV4.pack(
+        key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), err, kt, kh, vt, vh, kb, kch, vb, vch, tokens, hkv, dim, bs, nblk, dim // groups, _OUT_DTYPES[rt], 0))
+
+
+def _refuse_kv4(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, dtypes) -> None:
+    """Say what is wrong with the tensors of a 4-bit append or gather."""
+    if key.dtype not in dtypes:
+        raise ValueError(f"key must be one of {dtypes}, got {key.dtype}")
+    _dev(key, "key", key.dtype)
+    _dev(value, "value", key.dtype)
+    _dev(slot_mapping, "slot_mapping", torch.int32)
+    for t, n in ((key_cache, "key_cache"), (value_cache, "value_cache")):
+        _dev(t, n, torch.uint8)
+    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        _dev(t, n, torch.float16)
+    if error_count is not None:
+        _dev(error_count, "error_count", torch.int32)
+    if not _one_device(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale):
+        raise ValueError("the tensors must be on one device")
+    raise ValueError(
+        "4-bit caches: key and value [num_tokens, kv_heads, head_dim] with unit head-dim stride, slot_mapping "
+        "contiguous [num_tokens], pages [num_blocks, kv_heads, block_size, head_dim / 2] contiguous within a block "
+        f"and head, scales contiguous [num_blocks, kv_heads, groups, block_size, 2]; got {tuple(key.shape)}, "
+        f"{tuple(value.shape)}, {tuple(slot_mapping.shape)}, {tuple(key_cache.shape)}, {tuple(value_cache.shape)}, "
+        f"{tuple(k_scale.shape)}, {tuple(v_scale.shape)}")
+
+
+def kv4_append(key: torch.Tensor, value: torch.Tensor, slot_mapping: torch.Tensor, key_cache: torch.Tensor,
+               value_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+               error_count: torch.Tensor | None = None, stream: int | None = None) -> None:
+    """Quantise ``key[t]`` and ``value[t]``, ``[kv_heads, D]`` bf16 or fp16, to 4 bits at ``slot_mapping[t]``.
+
+    The pools are ``alloc_kv4_pools``'s. Slots as for ``kv_append``: negative ones
+    are skipped, those past the pool skipped and counted in ``error_count``; the
+    others have to differ. Element error: half a scale (``(max - min) / 30`` of
+    its group), and fp16's rounding of the group's bounds; values past fp16's
+    range saturate, and a group with a NaN or an infinity reads back as NaN.
+    """
+    a = _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count,
+                  (torch.bfloat16, torch.float16))
+    _launch("simpler_hip_kv4_append", a, key.device, stream)
+
+
+def kv4_gather(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, k_scale: torch.Tensor,
+               v_scale: torch.Tensor, key: torch.Tensor | None = None, value: torch.Tensor | None = None, *,
+               dtype: torch.dtype = torch.bfloat16, error_count: torch.Tensor | None = None,
+               stream: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows ``[num_tokens, kv_heads, D]`` of a 4-bit cache at ``slot_mapping``, as bf16, fp16 or fp32 ``(key, value)``.
+
+    Negative slots give zero rows; those past the pool too, counted in
+    ``error_count``. For what works on rows: attention of a prompt chunk over a
+    cached prefix, moving a sequence to another cache.
+    """
+    if key is None or value is None:
+        shape = (slot_mapping.shape[0], key_cache.shape[1], 2 * key_cache.shape[3])
+        key = torch.empty(shape, dtype=dtype, device=key_cache.device) if key is None else key
+        value = torch.empty(shape, dtype=dtype, device=key_cache.device) if value is None else value
+    a = _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count,
+                  (torch.bfloat16, torch.float16, torch.float32))
+    _launch("simpler_hip_kv4_gather", a, key.device, stream)
+    return key, value
+
+
+# ---------------------------------------------------------------------------
+# The prelude with rotary positions of several axes
+# ---------------------------------------------------------------------------
+
+_MROPE = struct.Struct("@14P9q11i4if")
+assert _MROPE.size <= ctypes.sizeof(_lib.QkNormMropeArgs) < _MROPE.size + 8
+
+
+def qk_norm_mrope_append(q_proj: torch.Tensor, k_proj: torch.Tensor, v_proj: torch.Tensor, positions: torch.Tensor,
+                         sections: list[int] | tuple[int, ...], rope_cos: torch.Tensor, rope_sin: torch.Tensor,
+                         slot_mapping: torch.Tensor | None, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                         num_heads: int, q_out: torch.Tensor | None = None, *, interleaved: bool = False,
+                         inv_rms: torch.Tensor | None = None, q_norm_weight: torch.Tensor | None = None,
+                         k_norm_weight: torch.Tensor | None = None, eps: float = EPS,
+                         error_count: torch.Tensor | None = None, stream: int | None = None) -> torch.Tensor:
+    """``qk_norm_rope_append`` with positions of several axes (time, height, width); returns ``q_out`` ``[T, Hq, D]``.
+
+    Pair i of a head (dims i and i + D/2) turns by the angle of its axis'
+    position, ``rope_cos/sin[positions[axis(i), t], (i, i + D/2)]``:
+    ``sections`` counts each axis' pairs, in order, or with ``interleaved`` pair i
+    has axis ``a = i % len(sections)`` where ``i < len(sections) * sections[a]``,
+    else axis 0. ``q_proj [T, Hq·D]``, ``k_proj``/``v_proj [T, Hkv·D]`` fp32, bf16 or
+    fp16 (rows may be parts of a wider projection), ``positions [axes, T]`` int32,
+    tables ``[max_position, D]`` fp32. ``inv_rms [T]`` and the norm weights ``[D]``
+    (fp32) are optional, each of them. Results are rounded to the caches' dtype,
+    bf16 or fp16. With ``slot_mapping=None`` key_cache and value_cache are rows
+    ``[T, Hkv, D]`` that are simply filled, as ``kv4_append`` and the decode's append
+    take them. Tokens whose position on axis 0 is negative are padding (zero q,
+    no rows written); other positions outside the tables count in ``error_count``.
+    """
+    tokens, dim = q_proj.shape[0], key_cache.shape[-1]
+    if slot_mapping is None:
+        if key_cache.dim() != 3 or value_cache.dim() != 3:
+            raise ValueError("without slot_mapping, key_cache and value_cache are rows [num_tokens, kv_heads, head_dim]")
+        if key_cache.shape[0] != tokens or value_cache.shape[0] != tokens:
+            raise ValueError("without slot_mapping, key_cache and value_cache have a row per token")
+        hkv, nblk, bs = key_cache.shape[1], 1, max(tokens, 1)
+        kst, vst = (8, *key_cache.stride()[:2]), (8, *value_cache.stride()[:2])  # one block: its stride is not used
+        unit = key_cache.stride(2) == 1 and value_cache.stride(2) == 1
+    else:
+        if key_cache.dim() != 4 or value_cache.dim() != 4:
+            raise ValueError("key_cache and value_cache must be [num_blocks, block_size, kv_heads, head_dim]")
+        nblk, bs, hkv = key_cache.shape[:3]
+        kst, vst = key_cache.stride()[:3], value_cache.stride()[:3]
+        unit = key_cache.stride(3) == 1 and value_cache.stride(3) == 1
+    dtype, proj, axes, i32, f32 = key_cache.dtype, q_proj.dtype, len(sections), torch.int32, torch.float32
+    if dtype not in (torch.bfloat16, torch.float16) or proj not in _OUT_DTYPES:
+        raise ValueError(f"caches must be bfloat16 or float16 and projections also or float32, got {dtype}, {proj}")
+    if value_cache.shape != key_cache.shape or not unit:
+        raise ValueError("value_cache must match key_cache, both with unit head-dim stride")
+    if not 1 <= axes <= 4 or sum(sections) * 2 != dim:
+        raise ValueError(f"sections must be one to four counts that sum to head_dim / 2 = {dim // 2}, got {sections}")
+    for t, n, w in ((q_proj, "q_proj", num_heads * dim), (k_proj, "k_proj", hkv * dim), (v_proj, "v_proj", hkv * dim)):
+        if t.dtype is not proj or not t.is_cuda or t.shape != (tokens, w) or t.stride(1) != 1:
+            raise ValueError(f"{n} must be a device {proj} [{tokens}, {w}] tensor with unit stride in its rows")
+    if positions.dtype is not i32 or not positions.is_cuda or positions.shape != (axes, tokens) \
+            or not positions.is_contiguous():
+        raise ValueError(f"positions must be a contiguous int32 device tensor [{axes}, {tokens}]")
+    if rope_cos.dim() != 2 or rope_cos.shape[1] != dim or rope_sin.shape != rope_cos.shape:
+        raise ValueError("rope tables must be [max_position, head_dim]")
+    small = [(rope_cos, "rope_cos", rope_cos.numel()), (rope_sin, "rope_sin", rope_cos.numel())]
+    small += [(t, n, k) for t, n, k in ((inv_rms, "inv_rms", tokens), (q_norm_weight, "q_norm_weight", dim),
+                                        (k_norm_weight, "k_norm_weight", dim)) if t is not None]
+    for t, n, k in small:
+        if t.dtype is not f32 or not t.is_cuda or not t.is_contiguous() or t.numel() != k:
+            raise ValueError(f"{n} must be a contiguous float32 device tensor of {k} elements")
+    if slot_mapping is not None and (slot_mapping.dtype is not i32 or not slot_mapping.is_cuda
+                                     or slot_mapping.shape != (tokens,) or not slot_mapping.is_contiguous()):
+        raise ValueError("slot_mapping must be a contiguous int32 device tensor [num_tokens]")
+    if error_count is not None and (error_count.dtype is not i32 or not error_count.is_cuda):
+        raise ValueError("error_count must be an int32 device tensor")
+    if not key_cache.is_cuda or not value_cache.is_cuda or value_cache.dtype is not dtype:
+        raise ValueError("key_cache and value_cache must be device tensors of one dtype")
+    if q_out is None:
+        q_out = torch.empty((tokens, num_heads, dim), dtype=dtype, device=q_proj.device)
+    elif q_out.dtype is not dtype or not q_out.is_cuda or not q_out.is_contiguous() or q_out.shape != (tokens, num_heads, dim):
+        raise ValueError(f"q_out must be a contiguous device {dtype} tensor [{tokens}, {num_heads}, {dim}]")
+    if not _one_device(q_proj, k_proj, v_proj, positions, rope_cos, rope_sin, key_cache, value_cache, q_out,
+                       *(t for t in (slot_mapping, inv_rms, q_norm_weight, k_norm_weight) if t is not None)):
+        raise ValueError("the tensors must be on one device")
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    row = lambda t: t.stride(0) if tokens > 1 else t.shape[1]  # noqa: E731
+    packed = _MROPE.pack(
+        q_proj.data_ptr(), k_proj.data_ptr(), v_proj.data_ptr(), ptr(inv_rms), ptr(q_norm_weight), ptr(k_norm_weight),
+        rope_cos.data_ptr(), rope_sin.data_ptr(), positions.data_ptr(), ptr(slot_mapping), q_out.data_ptr(),
+        key_cache.data_ptr(), value_cache.data_ptr(), ptr(error_count), row(q_proj), row(k_proj), row(v_proj),
+        *kst, *vst, tokens, num_heads, hkv, dim, bs, nblk, rope_cos.shape[0], _OUT_DTYPES[proj], _OUT_DTYPES[dtype],
+        axes, 1 if interleaved else 0, *sections, *([0] * (4 - axes)), eps)
+    a = _lib.QkNormMropeArgs.from_buffer_copy(packed.ljust(ctypes.sizeof(_lib.QkNormMropeArgs), b"\0"))
+    _launch("simpler_hip_qk_norm_mrope_append", a, q_proj.device, stream)
+    return q_out
+
+
+# ---------------------------------------------------------------------------
+# Block tables and slot maps of a step
+# ---------------------------------------------------------------------------
+
+
+class ReleasedBlocks(NamedTuple):
+    """What ``release_blocks`` returns: the step's lengths and free count."""
+
+    context_lens: torch.Tensor  # [B]
+    free_count: torch.Tensor  # [1]
+
+
+class StepSlots(NamedTuple):
+    """What ``assign_slots`` returns, all int32 on the device."""
+
+    slot_mapping: torch.Tensor  # [num_tokens]: -1 where a token has no place
+    positions: torch.Tensor  # [num_tokens]
+    requests: torch.Tensor  # [num_tokens]
+    starts: torch.Tensor  # [B + 1]: request b's tokens are starts[b] .. starts[b + 1]
+    context_lens: torch.Tensor  # [B]
+    granted: torch.Tensor  # [B]: new_lens, or 0 where refused
+    free_count: torch.Tensor  # [1]
+
+
+_RELEASE, _ASSIGN = struct.Struct("@8P4i"), struct.Struct("@13P5i")
+
+
+def _int32(t: torch.Tensor, name: str, shape: tuple[int, ...], at: int) -> int:
+    """Address of a contiguous int32 tensor of this shape on device ``at``."""
+    if t.dtype is not torch.int32 or not t.is_cuda or t.shape != shape or not t.is_contiguous() or t.get_device() != at:
+        raise ValueError(f"{name} must be a contiguous int32 tensor {list(shape)} on the block table's device, got "
+                         f"{t.dtype} {list(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _parts(sizes: tuple[int, ...], device: torch.device) -> list[torch.Tensor]:
+    """int32 tensors of these sizes in one allocation, each 16-byte aligned."""
+    starts, at = [], 0
+    for n in sizes:
+        starts.append(at)
+        at += (n + 3) // 4 * 4
+    buf = torch.empty(at, dtype=torch.int32, device=device)
+    return [buf.narrow(0, s, n) for s, n in zip(starts, sizes)]
+
+
+def release_blocks(ended: torch.Tensor, context_lens: torch.Tensor, block_table: torch.Tensor,
+                   free_blocks: torch.Tensor, free_count: torch.Tensor, block_size: int,
+                   error_count: torch.Tensor | None = None, stream: int | None = None) -> ReleasedBlocks:
+    """Return the blocks of the requests with ``ended[b] != 0`` to the free list.
+
+    The free ids are ``free_blocks[:free_count]`` (``free_blocks`` as long as the pool
+    has blocks, ``free_count [1]``); the ``ceil(context_lens[b] / block_size)`` ids of each ended
+    request's table row are put on top of them, request by request. Returns the
+    lengths (0 where ended) and the new count; nothing is read back to the host.
+    For requests that own their blocks alone: ids that two rows share would be
+    returned twice. Everything int32 and contiguous; at most 4096 requests.
+    """
+    (batch, width), device, at = block_table.shape, block_table.device, block_table.get_device()
+    inputs = (_int32(ended, "ended", (batch,), at), _int32(context_lens, "context_lens", (batch,), at),
+              _int32(block_table, "block_table", (batch, width), at),
+              _int32(free_blocks, "free_blocks", free_blocks.shape[:1], at), _int32(free_count, "free_count", (1,), at))
+    errors = 0 if error_count is None else _int32(error_count, "error_count", (1,), at)
+    lens_out, count_out = _parts((batch, 1), device)
+    a = _lib.ReleaseBlocksArgs.from_buffer_copy(_RELEASE.pack(
+        *inputs, lens_out.data_ptr(), count_out.data_ptr(), errors, batch, width, block_size, free_blocks.shape[0]))
+    _launch("simpler_hip_release_blocks", a, device, stream)
+    return ReleasedBlocks(lens_out, count_out)
+
+
+def assign_slots(new_lens: torch.Tensor, context_lens: torch.Tensor, block_table: torch.Tensor,
+                 free_blocks: torch.Tensor, free_count: torch.Tensor, block_size: int, num_tokens: int,
+                 error_count: torch.Tensor | None = None, stream: int | None = None) -> StepSlots:
+    """Blocks, positions and slots for a step's new tokens, built on the device.
+
+    Request b has ``context_lens[b]`` tokens cached and brings ``new_lens[b]`` (0, 1 or
+    a prompt's); the tokens of all requests are packed in request order, up to
+    ``num_tokens`` of them. ``block_table`` gets the blocks that are missing, in
+    place, from the top of the free list (``free_blocks[free_count - 1]`` first). The slots are
+    those that ``kv_append``, ``kv4_append`` and the preludes take (-1: no place), the
+    returned lengths those of the decode after the append. A request gets all of
+    its tokens or none: it is refused (``granted[b] == 0``, counted in ``error_count``)
+    where a length is negative, its tokens do not fit its table row or end past
+    ``num_tokens``, or the free list does not cover it and every earlier request.
+    Inputs stay as they are (the new lengths and count are outputs), so the same
+    call gives the same results again. Everything int32 and contiguous; at most
+    4096 requests.
+    """
+    if num_tokens < 0:
+        raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
+    (batch, width), device, at = block_table.shape, block_table.device, block_table.get_device()
+    inputs = (_int32(new_lens, "new_lens", (batch,), at), _int32(context_lens, "context_lens", (batch,), at),
+              _int32(block_table, "block_table", (batch, width), at),
+              _int32(free_blocks, "free_blocks", free_blocks.shape[:1], at), _int32(free_count, "free_count", (1,), at))
+    errors = 0 if error_count is None else _int32(error_count, "error_count", (1,), at)
+    parts = _parts(
+        (num_tokens, num_tokens, num_tokens, batch + 1, batch, batch, 1), device)
+    a = _lib.AssignSlotsArgs.from_buffer_copy(_ASSIGN.pack(
+        *inputs, *(t.data_ptr() for t in parts), errors, batch, width, block_size, free_blocks.shape[0],
+        num_tokens).ljust(ctypes.sizeof(_lib.AssignSlotsArgs), b"\0"))
+    _launch("simpler_hip_assign_slots", a, device, stream)
+    return StepSlots(*parts)

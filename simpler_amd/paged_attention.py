@@ -29,8 +29,8 @@ NATIVE_CALLABLE_NAME = "simpler_hip_paged_attention_decode"
 _OUT_DTYPES = {torch.float32: int(DataType.FLOAT32), torch.bfloat16: int(DataType.BFLOAT16),
                torch.float16: int(DataType.FLOAT16)}
 # element formats of query and caches (include/simpler_hip/pa_decode.h SIMPLER_HIP_KV_*):
-# bf16, fp8 E4M3FN caches with a bf16 query, fp16
-KV_BF16, KV_FP8_E4M3, KV_FP16 = 0, 1, 2
+# bf16, fp8 E4M3FN caches with a bf16 query, fp16, 4-bit pages with a bf16 or fp16 query
+KV_BF16, KV_FP8_E4M3, KV_FP16, KV_INT4_BF16, KV_INT4_FP16 = 0, 1, 2, 3, 4
 _FP8_DTYPES = (torch.float8_e4m3fn, torch.uint8)
 _ERRORS = {
     -1: "invalid argument (shape, dtype, stride or alignment)",
@@ -109,8 +109,43 @@ def _check(t: torch.Tensor, name: str, dtype: torch.dtype, ndims: tuple[int, ...
 
 
 # SimplerHipPaDecodeArgs as _lib.PaDecodeArgs lays it out
-_ARGS = struct.Struct("@6P6q10if3i2P")
+_ARGS = struct.Struct("@6P6q10if3i2P2i")
 assert _ARGS.size == ctypes.sizeof(_lib.PaDecodeArgs)
+
+
+def is_int4(key_cache: torch.Tensor, k_scale: torch.Tensor | None) -> bool:
+    """Whether caches with these scales are 4-bit pages (``kv_cache.alloc_kv4_pools``): uint8 with fp16 scales."""
+    return k_scale is not None and k_scale.dtype is torch.float16 and key_cache.dtype is torch.uint8
+
+
+def _plain_int4_args(query, key_cache, value_cache, block_table, context_lens, out, scale, causal, num_workers,
+                     k_scale, v_scale) -> _lib.PaDecodeArgs | None:
+    """``_plain_args`` for 4-bit pages."""
+    qs, (nblk, hkv, bs, row), (sn, sh, groups, sb, two) = query.shape, key_cache.shape, k_scale.shape
+    qt, ot = query.dtype, out.dtype
+    batch, q_len, (hq, dk) = qs[0], (qs[1] if len(qs) == 4 else 1), qs[-2:]
+    kb, kh, kr, k1 = key_cache.stride()
+    vb, vh, vr, v1 = value_cache.stride()
+    tb, width = block_table.shape
+    if not (
+        len(qs) in (3, 4) and (qt is torch.bfloat16 or qt is torch.float16) and (ot is torch.float32 or ot is qt)
+        and value_cache.dtype is torch.uint8 and v_scale.dtype is torch.float16 and 2 * row == dk
+        and value_cache.shape == key_cache.shape and v_scale.shape == k_scale.shape
+        and (sn, sh, sb, two) == (nblk, hkv, bs, 2) and dk % groups == 0 and k1 == 1 and v1 == 1 and kr == row
+        and vr == row and out.shape == qs and tb == batch and context_lens.shape == (batch,)
+        and block_table.dtype is torch.int32 and context_lens.dtype is torch.int32 and query.is_cuda
+        and key_cache.is_cuda and value_cache.is_cuda and k_scale.is_cuda and v_scale.is_cuda and block_table.is_cuda
+        and context_lens.is_cuda and out.is_cuda and query.is_contiguous() and out.is_contiguous()
+        and block_table.is_contiguous() and context_lens.is_contiguous() and k_scale.is_contiguous()
+        and v_scale.is_contiguous()
+    ):
+        return None
+    return _lib.PaDecodeArgs.from_buffer_copy(_ARGS.pack(
+        query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
+        context_lens.data_ptr(), out.data_ptr(), kb, row, kh, vb, row, vh, batch, q_len, hq, hkv, dk, dk, bs, width,
+        nblk, _OUT_DTYPES[ot], scale, 1 if causal else 0, num_workers,
+        KV_INT4_BF16 if qt is torch.bfloat16 else KV_INT4_FP16, k_scale.data_ptr(), v_scale.data_ptr(), dk // groups,
+        0))
 
 
 def _plain_args(query, key_cache, value_cache, block_table, context_lens, out, scale, causal, num_workers, k_scale,
@@ -120,6 +155,9 @@ def _plain_args(query, key_cache, value_cache, block_table, context_lens, out, s
     about as long as the call takes the host); None leaves the call to the
     checks, which name what is wrong."""
     try:
+        if is_int4(key_cache, k_scale):
+            return _plain_int4_args(query, key_cache, value_cache, block_table, context_lens, out, scale, causal,
+                                    num_workers, k_scale, v_scale)
         qs, (nblk, bs, hkv, dk), (vnb, vbs, vhkv, dv) = query.shape, key_cache.shape, value_cache.shape
         qt, kt, ot = query.dtype, key_cache.dtype, out.dtype
         if len(qs) == 3:
@@ -153,7 +191,7 @@ def _plain_args(query, key_cache, value_cache, block_table, context_lens, out, s
         return _lib.PaDecodeArgs.from_buffer_copy(_ARGS.pack(
             query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
             context_lens.data_ptr(), out.data_ptr(), kb, ktk, kh, vb, vtk, vh, batch, q_len, hq, hkv, dk, dv, bs,
-            width, nblk, _OUT_DTYPES[ot], scale, 1 if causal else 0, num_workers, fmt, kp, vp))
+            width, nblk, _OUT_DTYPES[ot], scale, 1 if causal else 0, num_workers, fmt, kp, vp, 0, 0))
     except (AttributeError, TypeError, ValueError, struct.error, OverflowError):
         return None
 
@@ -178,11 +216,17 @@ def make_args(
     (or uint8 holding E4M3FN bytes) with ``k_scale``/``v_scale`` fp32
     ``[num_blocks, num_kv_heads]``: element (blk, t, h, d) stands for
     ``float(cache[blk, t, h, d]) * scale[blk, h]``.
+
+    4-bit caches: uint8 pages and fp16 scales as ``kv_cache.alloc_kv4_pools``
+    lays them out (``[num_blocks, kv_heads, block_size, head_dim / 2]`` and
+    ``[num_blocks, kv_heads, groups, block_size, 2]``).
     """
     plain = _plain_args(query, key_cache, value_cache, block_table, context_lens, out, scale, causal, num_workers,
                         k_scale, v_scale)
     if plain is not None:
         return plain
+    if is_int4(key_cache, k_scale):
+        _refuse_int4(query, key_cache, value_cache, block_table, context_lens, out, k_scale, v_scale)
     fp8 = key_cache.dtype in _FP8_DTYPES
     fp16 = query.dtype == torch.float16
     kv_dtype = key_cache.dtype if fp8 else (torch.float16 if fp16 else torch.bfloat16)
@@ -245,6 +289,39 @@ def make_args(
     elif fp16:
         a.kv_format = KV_FP16
     return a
+
+
+def _refuse_int4(query, key_cache, value_cache, block_table, context_lens, out, k_scale, v_scale) -> None:
+    """Say what is wrong with 4-bit decode arguments that ``_plain_int4_args`` did not take."""
+    half = torch.float16 if query.dtype == torch.float16 else torch.bfloat16
+    _check(query, "query", half, (3, 4))
+    _check(key_cache, "key_cache", torch.uint8, (4,))
+    _check(value_cache, "value_cache", torch.uint8, (4,))
+    _check(k_scale, "k_scale", torch.float16, (5,))
+    _check(v_scale, "v_scale", torch.float16, (5,))
+    _check(block_table, "block_table", torch.int32, (2,))
+    _check(context_lens, "context_lens", torch.int32, (1,))
+    if out.dtype not in (torch.float32, half):
+        raise ValueError(f"out must be torch.float32 or {half} for a {half} query, got {out.dtype}")
+    for name, t in (("query", query), ("block_table", block_table), ("context_lens", context_lens), ("out", out),
+                    ("k_scale", k_scale), ("v_scale", v_scale)):
+        if not t.is_contiguous() or t.device.type != "cuda":
+            raise ValueError(f"{name} must be a contiguous device tensor")
+    nblk, hkv, bs, row = key_cache.shape
+    if value_cache.shape != key_cache.shape or 2 * row != query.shape[-1]:
+        raise ValueError("key_cache/value_cache must be [num_blocks, kv_heads, block_size, head_dim / 2] for the query")
+    for name, t in (("key_cache", key_cache), ("value_cache", value_cache)):
+        if t.stride()[2:] != (row, 1):
+            raise ValueError(f"{name}: a block and kv head's page must be contiguous")
+    if v_scale.shape != k_scale.shape or k_scale.shape != (nblk, hkv, k_scale.shape[2], bs, 2):
+        raise ValueError("k_scale/v_scale must be [num_blocks, kv_heads, groups, block_size, 2]")
+    if query.shape[-1] % k_scale.shape[2]:
+        raise ValueError("the head dim must be a multiple of the scales' groups")
+    if out.shape != query.shape:
+        raise ValueError(f"out must have shape {tuple(query.shape)}, got {tuple(out.shape)}")
+    if block_table.shape[0] != query.shape[0] or context_lens.shape != query.shape[:1]:
+        raise ValueError("block_table/context_lens batch does not match the query")
+    raise ValueError("scale and num_workers must be numbers")
 
 
 PHASE_MAIN, PHASE_MERGE = 1, 2
@@ -324,7 +401,7 @@ def append_tensors(args: _lib.PaDecodeArgs, query: torch.Tensor, key_cache: torc
     ``key_new`` ``[B, q_len, Hkv, Dk]`` (or ``[B, Hkv, Dk]`` for q_len 1) and
     ``value_new`` ``[..., Dv]`` contiguous, of the caches' dtype; ``value_new`` is
     ``None`` exactly when ``value_cache`` is a view of ``key_cache`` (MLA)."""
-    kv_dtype = key_cache.dtype
+    kv_dtype = query.dtype if args.kv_format in (KV_INT4_BF16, KV_INT4_FP16) else key_cache.dtype
     q_len = args.q_len
     mla = value_cache.data_ptr() == key_cache.data_ptr()
     for name, t, d in (("key_new", key_new, args.head_dim_k), ("value_new", value_new, args.head_dim_v)):
@@ -363,13 +440,15 @@ def paged_attention_decode(
     writes FLOAT32 output (``paged_attention_orch.cpp:130``); BFLOAT16 (bf16
     inputs) or FLOAT16 (fp16 inputs) is also accepted. Query and caches are
     bfloat16, or float16 (the reference's GQA cases). ``value_cache`` may be a
-    view of ``key_cache`` (MLA: V = K[..., :Dv], bf16).
+    view of ``key_cache`` (MLA: V = K[..., :Dv], bf16). With uint8 pages and fp16
+    ``k_scale``/``v_scale`` (``kv_cache.alloc_kv4_pools``) the caches hold 4 bits
+    per value. A row that sees no token is 0.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(query.shape[-1])
     if out is None:
-        shape = (*query.shape[:-1], value_cache.shape[-1])
-        out = torch.empty(shape, dtype=out_dtype, device=query.device)
+        dv = query.shape[-1] if is_int4(key_cache, k_scale) else value_cache.shape[-1]
+        out = torch.empty((*query.shape[:-1], dv), dtype=out_dtype, device=query.device)
     args = make_args(
         query, key_cache, value_cache, block_table, context_lens, out, scale,
         causal=causal, num_workers=num_workers, k_scale=k_scale, v_scale=v_scale,
@@ -392,6 +471,8 @@ def paged_attention_decode_append(
     causal: bool = False,
     out_dtype: torch.dtype = torch.float32,
     num_workers: int = 0,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """KV-cache append fused into the decode (``simpler_hip_pa_decode_append``).
 
@@ -401,15 +482,17 @@ def paged_attention_decode_append(
     the caches at ``block_table[b, p // block_size]``, row ``p % block_size``, and
     the decode attends over them, as ``kv_append`` with that slot mapping
     followed by ``paged_attention_decode`` would. ``value_new`` is ``None`` for
-    MLA (V is a prefix of the K row). bf16 or fp16; q_len <= 16.
+    MLA (V is a prefix of the K row). bf16 or fp16; q_len <= 16. With 4-bit caches
+    (``k_scale``/``v_scale`` as for the decode) the rows, of the query's type, are
+    appended as by ``kv4_append``.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(query.shape[-1])
     if out is None:
-        shape = (*query.shape[:-1], value_cache.shape[-1])
-        out = torch.empty(shape, dtype=out_dtype, device=query.device)
+        dv = query.shape[-1] if is_int4(key_cache, k_scale) else value_cache.shape[-1]
+        out = torch.empty((*query.shape[:-1], dv), dtype=out_dtype, device=query.device)
     args = make_args(query, key_cache, value_cache, block_table, context_lens, out, scale, causal=causal,
-                     num_workers=num_workers)
+                     num_workers=num_workers, k_scale=k_scale, v_scale=v_scale)
     append_tensors(args, query, key_cache, value_cache, key_new, value_new)
     launch(args, query.device, key_new=key_new, value_new=value_new)
     return out

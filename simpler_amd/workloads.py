@@ -148,6 +148,37 @@ def dequantize_kv_fp8(cache8: torch.Tensor, scale: torch.Tensor) -> torch.Tensor
     return cache8.float() * scale[:, None, :, None].float()
 
 
+def quantize_kv4(rows: torch.Tensor, group: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """16-bit rows ``[..., D]`` -> 4-bit codes ``[..., D]`` (uint8 0..15), scale and
+    zero ``[..., D / group]`` fp16, as ``include/simpler_hip/kv_cache.h`` defines
+    them (in torch; the device path is ``kv_cache.kv4_append``)."""
+    x = rows.unflatten(-1, (-1, group)).float()
+    lo, hi = x.amin(-1), x.amax(-1)
+    bad = ~torch.isfinite(x).all(-1)
+    z = lo.clamp(-65504.0, 65504.0).half().masked_fill(bad, float("nan"))
+    s = ((hi - lo) / 15.0).clamp(max=65504.0).half().masked_fill(bad, float("nan"))
+    s64 = s.double()[..., None]
+    c = ((x.double() - z.double()[..., None]) / torch.where(s64 > 0, s64, 1.0)).round().clamp(0, 15)
+    return torch.where(s64 > 0, c, 0.0).nan_to_num(0.0).to(torch.uint8).flatten(-2), s, z
+
+
+def dequantize_kv4(codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor) -> torch.Tensor:
+    """fp64 values that ``quantize_kv4``'s output stands for: ``code * scale + zero``."""
+    c = codes.unflatten(-1, (scale.shape[-1], -1)).double()
+    return (c * scale.double()[..., None] + zero.double()[..., None]).flatten(-2)
+
+
+def pack_kv4_pages(codes: torch.Tensor, value: bool) -> torch.Tensor:
+    """Codes ``[num_blocks, kv_heads, block_size, D]`` -> uint8 pages ``[..., block_size, D / 2]`` of a K or V pool."""
+    n, hkv, bs, dim = codes.shape
+    if not value:  # word (D/32) a + j, nibble i: dim 32 j + 8 a + i
+        nib = codes.view(n, hkv, bs, dim // 32, 4, 8).transpose(3, 4).reshape(n, hkv, bs, dim // 2, 2)
+    else:  # row 4 g + 2 b + r, dim 64 h + 32 u + 2 l + v -> [g, l, b, h, r, u, v]
+        nib = codes.view(n, hkv, bs // 4, 2, 2, dim // 64, 2, 16, 2).permute(0, 1, 2, 7, 3, 5, 4, 6, 8)
+        nib = nib.reshape(n, hkv, bs, dim // 2, 2)
+    return nib[..., 0] | (nib[..., 1] << 4)
+
+
 def make_case(cfg: DecodeConfig | str, seed: int | None = None, *, ctx_override: list[int] | None = None,
               batch_override: int | None = None) -> DecodeCase:
     """Generate one seeded case on the CPU (deterministic across machines)."""
