@@ -64,7 +64,7 @@ typedef struct SimplerHipAssignSlotsArgs {
     int32_t *granted;            /* [batch]: new_lens, or 0 where refused */
     int32_t *free_count_out;     /* [1] */
     int32_t *error_count;        /* or NULL: refused requests are counted */
-    int32_t batch, max_blocks_per_seq, block_size, capacity, num_tokens;
+    int32_t batch, max_blocks_per_seq, block_size, capacity, num_tokens, reserved;
 } SimplerHipAssignSlotsArgs;
 
 /* The tokens of all requests, packed in request order (request b's are the

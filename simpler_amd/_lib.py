@@ -155,7 +155,8 @@ class AssignSlotsArgs(ctypes.Structure):
         *[(n, ctypes.c_void_p) for n in ("new_lens", "context_lens", "block_table", "free_blocks", "free_count",
                                           "slot_mapping", "positions", "requests", "starts", "context_lens_out",
                                           "granted", "free_count_out", "error_count")],
-        *[(n, ctypes.c_int32) for n in ("batch", "max_blocks_per_seq", "block_size", "capacity", "num_tokens")],
+        *[(n, ctypes.c_int32) for n in ("batch", "max_blocks_per_seq", "block_size", "capacity", "num_tokens",
+                                         "reserved")],
     ]
 
 
@@ -185,12 +186,13 @@ SIGNATURES: dict[str, tuple] = {
     # include/simpler_hip/kv_cache.h
     "simpler_hip_kv_append": (_I, [ctypes.POINTER(KvAppendArgs), _VP]),
     "simpler_hip_qk_norm_rope_append": (_I, [ctypes.POINTER(QkNormRopeAppendArgs), _VP]),
-    "simpler_hip_kv4_append": (_I, [ctypes.POINTER(Kv4Args), _VP]),
-    "simpler_hip_kv4_gather": (_I, [ctypes.POINTER(Kv4Args), _VP]),
-    "simpler_hip_qk_norm_mrope_append": (_I, [ctypes.POINTER(QkNormMropeArgs), _VP]),
+    # (their args as void*: packed bytes, or a reference to the structure above)
+    "simpler_hip_kv4_append": (_I, [_VP, _VP]),
+    "simpler_hip_kv4_gather": (_I, [_VP, _VP]),
+    "simpler_hip_qk_norm_mrope_append": (_I, [_VP, _VP]),
     # include/simpler_hip/step_plan.h
-    "simpler_hip_release_blocks": (_I, [ctypes.POINTER(ReleaseBlocksArgs), _VP]),
-    "simpler_hip_assign_slots": (_I, [ctypes.POINTER(AssignSlotsArgs), _VP]),
+    "simpler_hip_release_blocks": (_I, [_VP, _VP]),
+    "simpler_hip_assign_slots": (_I, [_VP, _VP]),
     # include/simpler_hip/pto_runtime_c_api.h
     "get_pipeline_contract": (_VP, []),
     "get_runtime_size": (_SZ, []),

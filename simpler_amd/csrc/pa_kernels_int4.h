@@ -48,18 +48,19 @@ __device__ __forceinline__ u32x4_t nibbles_subnormal(const unsigned x) {
 }
 
 // The same pairs as fp16 integers c - 8, exact: 1024 + c - 1032 and
-// (1024 + 16 c) / 16 - 72.
-__device__ __forceinline__ u32x4_t nibbles_centred(const unsigned x) {
+// (1024 + 16 c) / 16 - 72. The masks and the 1024s come in registers (`low`,
+// `high`, `k1024`), for one v_and_or_b32 per pair: as literals
+// they take an and and an or.
+__device__ __forceinline__ u32x4_t nibbles_centred(const unsigned x, const unsigned low, const unsigned high,
+                                                   const unsigned k1024) {
     const f16x2_t off = (f16x2_t){(_Float16)-1032.f, (_Float16)-1032.f};
     const f16x2_t sixteenth = (f16x2_t){(_Float16)0.0625f, (_Float16)0.0625f};
     const f16x2_t off16 = (f16x2_t){(_Float16)-72.f, (_Float16)-72.f};
     const unsigned y = x >> 8;
-    const f16x2_t a = __builtin_bit_cast(f16x2_t, (x & 0x000f000fu) | 0x64006400u) + off;
-    const f16x2_t b = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, (x & 0x00f000f0u) | 0x64006400u),
-                                                sixteenth, off16);
-    const f16x2_t c = __builtin_bit_cast(f16x2_t, (y & 0x000f000fu) | 0x64006400u) + off;
-    const f16x2_t d = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, (y & 0x00f000f0u) | 0x64006400u),
-                                                sixteenth, off16);
+    const f16x2_t a = __builtin_bit_cast(f16x2_t, (x & low) | k1024) + off;
+    const f16x2_t b = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, (x & high) | k1024), sixteenth, off16);
+    const f16x2_t c = __builtin_bit_cast(f16x2_t, (y & low) | k1024) + off;
+    const f16x2_t d = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, (y & high) | k1024), sixteenth, off16);
     return (u32x4_t){__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, c),
                      __builtin_bit_cast(unsigned, d)};
 }
@@ -107,13 +108,18 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
     constexpr int DH = D / 64;    // words per lane, tile and token pair of V
     // Where registers are short the tiles' work is kept apart: the scheduler
     // would otherwise mix it and spill.
-    constexpr bool kTight = RTW * D * (NG + 1) > 384;
+    constexpr bool kTight = true;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     constexpr float kSlack = 8.f;  // a score may pass the frame by 2^kSlack
     static_assert(D % 64 == 0 && KS % NG == 0, "head dims: multiples of 64, groups of whole k-steps");
     const int lane = threadIdx.x & 63, qd = lane >> 4, pc = lane & 15;
     const int bs = P.block_size, sh = __builtin_ctz(bs);
     const bool f16 = P.half16;
+    // constants of the conversions, kept in registers
+    unsigned low = 0x000f000fu, high = 0x00f000f0u, k1024 = 0x64006400u;
+    asm volatile("" : "+s"(low), "+s"(high));
+    asm volatile("" : "+v"(k1024));
+    auto centred = [&](const unsigned x) { return nibbles_centred(x, low, high, k1024); };
 
     // ---- Q: row pc of each row tile, in the codes' nibble order, exponent-aligned ----
     u32x4_t qv[RTW][KS];
@@ -134,14 +140,22 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
             rowlim[r] = min(seg_end, P.causal ? ctx - (P.q_len - 1 - i) : ctx);
         }
         float f[KS][8], amax = 0.f;
+        if (f16) {
+#pragma unroll
+            for (int j = 0; j < KS; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[j][2 * i] = half_lo(raw[j][i]), f[j][2 * i + 1] = half_hi(raw[j][i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < KS; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    f[j][2 * i] = __uint_as_float(raw[j][i] << 16), f[j][2 * i + 1] = __uint_as_float(raw[j][i] & 0xffff0000u);
+        }
 #pragma unroll
         for (int j = 0; j < KS; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f[j][2 * i] = f16 ? half_lo(raw[j][i]) : __uint_as_float(raw[j][i] << 16);
-                f[j][2 * i + 1] = f16 ? half_hi(raw[j][i]) : __uint_as_float(raw[j][i] & 0xffff0000u);
-                amax = fmaxf(amax, fmaxf(fabsf(f[j][2 * i]), fabsf(f[j][2 * i + 1])));
-            }
+            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[j][i]));
         amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
         amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
         // the row times 2^(140 - eb): its largest element in [2^13, 2^14)
@@ -319,7 +333,7 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
                 f32x4_t dot[RTW];
 #pragma unroll
                 for (int j = g * GM; j < (g + 1) * GM; ++j) {
-                    const u32x4_t a = EXACT ? nibbles_centred(kreg[t][j]) : nibbles_subnormal(kreg[t][j]);
+                    const u32x4_t a = EXACT ? centred(kreg[t][j]) : nibbles_subnormal(kreg[t][j]);
 #pragma unroll
                     for (int r = 0; r < RTW; ++r)
                         dot[r] = Elem<_Float16>::mma32(a, qv[r][j],
@@ -331,7 +345,8 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
                 for (int r = 0; r < RTW; ++r)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float zz = g == 0 ? z[e] * zq[r][g] : __builtin_fmaf(z[e], zq[r][g], y[r][t][e]);
+                        // (adding 0 in a fused form takes fp16 operands as they are)
+                        const float zz = __builtin_fmaf(z[e], zq[r][g], g == 0 ? 0.f : y[r][t][e]);
                         y[r][t][e] = __builtin_fmaf(s[e], dot[r][e], zz);
                     }
             }
@@ -419,7 +434,7 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
                         float v[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            v[e] = p[r][i][e] * s[e];
+                            v[e] = __builtin_fmaf(p[r][i][e], s[e], 0.f);
                             zacc[r][g] = __builtin_fmaf(p[r][i][e], z[e], zacc[r][g]);
                         }
                         ps[r][i] = (u32x2_t){Elem<_Float16>::pack2(v[0], v[1]), Elem<_Float16>::pack2(v[2], v[3])};
@@ -433,8 +448,8 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
 #pragma unroll
                 for (int h = 0; h < DH; ++h) {
                     if (4 * h + 3 < g * GT || 4 * h >= (g + 1) * GT) continue;  // no dim tile of this group
-                    const u32x4_t a = nibbles_centred(vreg[t][h]), c = nibbles_centred(vreg[t][DH + h]);
-                    const u32x4_t a2 = nibbles_centred(vreg[t + 1][h]), c2 = nibbles_centred(vreg[t + 1][DH + h]);
+                    const u32x4_t a = centred(vreg[t][h]), c = centred(vreg[t][DH + h]);
+                    const u32x4_t a2 = centred(vreg[t + 1][h]), c2 = centred(vreg[t + 1][DH + h]);
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
                         const int j = 4 * h + n;

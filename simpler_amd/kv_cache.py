@@ -268,18 +268,21 @@ def prelude_args(q_proj: torch.Tensor, k_proj: torch.Tensor, v_proj: torch.Tenso
     return a
 
 
-def _launch(name: str, args: ctypes.Structure, device: torch.device, stream: int | None) -> None:
-    """Run the C entry ``name`` on ``stream`` (default: torch's current one of ``device``), with that device current."""
+def _launch(name: str, packed: bytes, device: torch.device, stream: int | None) -> None:
+    """Run the C entry ``name`` on packed args and ``stream`` (default: torch's current one of ``device``), with
+    that device current."""
     fn = getattr(_lib.lib(), name)
-    if stream is None:
-        stream = _current_stream(device)
-    if device.index is None or device.index == torch.cuda.current_device():
-        rc = fn(ctypes.byref(args), stream)
+    at = device.index
+    if at is None or at == _current_device():
+        rc = fn(packed, _current_stream(device) if stream is None else stream)
     else:
         with torch.cuda.device(device):
-            rc = fn(ctypes.byref(args), stream)
+            rc = fn(packed, _current_stream(device) if stream is None else stream)
     if rc != 0:
         raise PagedAttentionError(rc, name)
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 # ---------------------------------------------------------------------------
@@ -333,18 +336,34 @@ def _one_device(first: torch.Tensor, *others: torch.Tensor) -> bool:
 # SimplerHipKv4Args as _lib.Kv4Args lays it out
 _KV4 = struct.Struct("@8P8q8i")
 assert _KV4.size == ctypes.sizeof(_lib.Kv4Args)
+_HALVES = (torch.bfloat16, torch.float16)
+_ROWS = (*_HALVES, torch.float32)
 
 
-def _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, dtypes) -> _lib.Kv4Args:
-    """Check the tensors of a 4-bit append or gather (rows of one of ``dtypes``) and fill the C args."""
-    rt = key.dtype
-    tokens, hkv, dim = key.shape
-    nblk, chkv, bs, row = key_cache.shape
+def _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, dtypes) -> bytes:
+    """Check the tensors of a 4-bit append or gather (rows of one of ``dtypes``) and pack the C args, in one pass
+    over the tensors' attributes (a small append takes the device less time than its checks the host)."""
+    rt, shape, pages, scales, at = key.dtype, key.shape, key_cache.shape, k_scale.shape, key.get_device()
+    tokens, hkv, dim = shape
+    nblk, chkv, bs, row = pages
+    groups = scales[2]
     kt, kh, k1 = key.stride()
     vt, vh, v1 = value.stride()
     kb, kch, kcr, kc1 = key_cache.stride()
     vb, vch, vcr, vc1 = value_cache.stride()
-    groups = k_scale.shape[2]
+    if not (
+        rt in dtypes and value.dtype is rt and value.shape == shape and k1 == 1 and v1 == 1
+        and key_cache.dtype is torch.uint8 and value_cache.dtype is torch.uint8 and value_cache.shape == pages
+        and chkv == hkv and 2 * row == dim and kcr == row and kc1 == 1 and vcr == row and vc1 == 1
+        and k_scale.dtype is torch.float16 and v_scale.dtype is torch.float16 and scales == (nblk, hkv, groups, bs, 2)
+        and v_scale.shape == scales and k_scale.is_contiguous() and v_scale.is_contiguous()
+        and groups > 0 and dim % groups == 0 and slot_mapping.dtype is torch.int32 and slot_mapping.shape == (tokens,)
+        and slot_mapping.is_contiguous() and key.is_cuda and value.get_device() == at and slot_mapping.get_device() == at
+        and key_cache.get_device() == at and value_cache.get_device() == at and k_scale.get_device() == at
+        and v_scale.get_device() == at
+        and (error_count is None or (error_count.dtype is torch.int32 and error_count.get_device() == at))
+    ):
+        _refuse_kv4(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, dtypes)
     if tokens <= 1:  # strides of dims of one element say nothing
         kt = vt = 8
     if hkv == 1:
@@ -352,23 +371,10 @@ def _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale
         kch = vch = 16
     if nblk == 1:
         kb = vb = 16
-    err = 0 if error_count is None else error_count.data_ptr()
-    u8, f16, i32 = torch.uint8, torch.float16, torch.int32
-    if not (
-        rt in dtypes and value.dtype is rt and value.shape == key.shape and k1 == 1 and v1 == 1
-        and key_cache.dtype is u8 and value_cache.dtype is u8 and value_cache.shape == key_cache.shape
-        and chkv == hkv and 2 * row == dim and kcr == row and kc1 == 1 and vcr == row and vc1 == 1
-        and k_scale.dtype is f16 and v_scale.dtype is f16 and k_scale.shape == (nblk, hkv, groups, bs, 2)
-        and v_scale.shape == k_scale.shape and k_scale.is_contiguous() and v_scale.is_contiguous()
-        and groups > 0 and dim % groups == 0 and slot_mapping.dtype is i32 and slot_mapping.shape == (tokens,)
-        and slot_mapping.is_contiguous() and key.is_cuda
-        and (error_count is None or (error_count.dtype is i32 and error_count.is_cuda))
-        and _one_device(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale)
-    ):
-        _refuse_kv4(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, dtypes)
-    return _lib.Kv4Args.from_buffer_copy(_KV4.pack(
+    return _KV4.pack(
         key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
-        k_scale.data_ptr(), v_scale.data_ptr(), err, kt, kh, vt, vh, kb, kch, vb, vch, tokens, hkv, dim, bs, nblk, dim // groups, _OUT_DTYPES[rt], 0))
+        k_scale.data_ptr(), v_scale.data_ptr(), 0 if error_count is None else error_count.data_ptr(), kt, kh, vt, vh,
+        kb, kch, vb, vch, tokens, hkv, dim, bs, nblk, dim // groups, _OUT_DTYPES[rt], 0)
 
 
 def _refuse_kv4(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, dtypes) -> None:
@@ -405,8 +411,7 @@ def kv4_append(key: torch.Tensor, value: torch.Tensor, slot_mapping: torch.Tenso
     its group), and fp16's rounding of the group's bounds; values past fp16's
     range saturate, and a group with a NaN or an infinity reads back as NaN.
     """
-    a = _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count,
-                  (torch.bfloat16, torch.float16))
+    a = _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, _HALVES)
     _launch("simpler_hip_kv4_append", a, key.device, stream)
 
 
@@ -421,11 +426,10 @@ def kv4_gather(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_cache:
     cached prefix, moving a sequence to another cache.
     """
     if key is None or value is None:
-        shape = (slot_mapping.shape[0], key_cache.shape[1], 2 * key_cache.shape[3])
-        key = torch.empty(shape, dtype=dtype, device=key_cache.device) if key is None else key
-        value = torch.empty(shape, dtype=dtype, device=key_cache.device) if value is None else value
-    a = _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count,
-                  (torch.bfloat16, torch.float16, torch.float32))
+        rows = torch.empty((2, slot_mapping.shape[0], key_cache.shape[1], 2 * key_cache.shape[3]), dtype=dtype,
+                           device=key_cache.device).unbind()
+        key, value = (rows[0] if key is None else key), (rows[1] if value is None else value)
+    a = _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, _ROWS)
     _launch("simpler_hip_kv4_gather", a, key.device, stream)
     return key, value
 
@@ -434,8 +438,9 @@ def kv4_gather(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_cache:
 # The prelude with rotary positions of several axes
 # ---------------------------------------------------------------------------
 
+# SimplerHipQkNormMropeArgs as _lib.QkNormMropeArgs lays it out
 _MROPE = struct.Struct("@14P9q11i4if")
-assert _MROPE.size <= ctypes.sizeof(_lib.QkNormMropeArgs) < _MROPE.size + 8
+assert _MROPE.size == ctypes.sizeof(_lib.QkNormMropeArgs)
 
 
 def qk_norm_mrope_append(q_proj: torch.Tensor, k_proj: torch.Tensor, v_proj: torch.Tensor, positions: torch.Tensor,
@@ -461,66 +466,94 @@ def qk_norm_mrope_append(q_proj: torch.Tensor, k_proj: torch.Tensor, v_proj: tor
     no rows written); other positions outside the tables count in ``error_count``.
     """
     tokens, dim = q_proj.shape[0], key_cache.shape[-1]
-    if slot_mapping is None:
-        if key_cache.dim() != 3 or value_cache.dim() != 3:
-            raise ValueError("without slot_mapping, key_cache and value_cache are rows [num_tokens, kv_heads, head_dim]")
-        if key_cache.shape[0] != tokens or value_cache.shape[0] != tokens:
-            raise ValueError("without slot_mapping, key_cache and value_cache have a row per token")
-        hkv, nblk, bs = key_cache.shape[1], 1, max(tokens, 1)
-        kst, vst = (8, *key_cache.stride()[:2]), (8, *value_cache.stride()[:2])  # one block: its stride is not used
-        unit = key_cache.stride(2) == 1 and value_cache.stride(2) == 1
+    kst, vst, shape, dtype = key_cache.stride(), value_cache.stride(), key_cache.shape, key_cache.dtype
+    if slot_mapping is None and len(shape) == 3:  # rows: one block, whose stride is not used
+        nblk, bs, hkv, kst, vst = 1, max(tokens, 1), shape[1], (8, *kst), (8, *vst)
+        paged = shape[0] == tokens
     else:
-        if key_cache.dim() != 4 or value_cache.dim() != 4:
-            raise ValueError("key_cache and value_cache must be [num_blocks, block_size, kv_heads, head_dim]")
-        nblk, bs, hkv = key_cache.shape[:3]
-        kst, vst = key_cache.stride()[:3], value_cache.stride()[:3]
-        unit = key_cache.stride(3) == 1 and value_cache.stride(3) == 1
-    dtype, proj, axes, i32, f32 = key_cache.dtype, q_proj.dtype, len(sections), torch.int32, torch.float32
-    if dtype not in (torch.bfloat16, torch.float16) or proj not in _OUT_DTYPES:
+        paged = slot_mapping is not None and len(shape) == 4
+        nblk, bs, hkv = shape[:3]
+    proj, axes, at = q_proj.dtype, len(sections), q_proj.get_device()
+    qs, ks, vs = q_proj.stride(), k_proj.stride(), v_proj.stride()
+    i32, f32, rope = torch.int32, torch.float32, rope_cos.shape
+    if not (
+        paged and dtype in _HALVES and proj in _OUT_DTYPES and value_cache.dtype is dtype and value_cache.shape == shape
+        and kst[-1] == 1 and vst[-1] == 1 and 1 <= axes <= 4 and 2 * sum(sections) == dim
+        and q_proj.shape == (tokens, num_heads * dim) and k_proj.shape == (tokens, hkv * dim)
+        and v_proj.shape == k_proj.shape and k_proj.dtype is proj and v_proj.dtype is proj
+        and qs[1] == 1 and ks[1] == 1 and vs[1] == 1 and positions.dtype is i32 and positions.shape == (axes, tokens)
+        and positions.is_contiguous() and len(rope) == 2 and rope[1] == dim and rope_sin.shape == rope
+        and rope_cos.dtype is f32 and rope_sin.dtype is f32 and rope_cos.is_contiguous() and rope_sin.is_contiguous()
+        and (q_out is None or (q_out.dtype is dtype and q_out.shape == (tokens, num_heads, dim)
+                               and q_out.is_contiguous() and q_out.get_device() == at))
+        and q_proj.is_cuda and k_proj.get_device() == at and v_proj.get_device() == at and positions.get_device() == at
+        and rope_cos.get_device() == at and rope_sin.get_device() == at and key_cache.get_device() == at
+        and value_cache.get_device() == at
+        and (slot_mapping is None or (slot_mapping.dtype is i32 and slot_mapping.shape == (tokens,)
+                                      and slot_mapping.is_contiguous() and slot_mapping.get_device() == at))
+        and (inv_rms is None or _vector(inv_rms, tokens, at)) and (q_norm_weight is None or _vector(q_norm_weight, dim, at))
+        and (k_norm_weight is None or _vector(k_norm_weight, dim, at))
+        and (error_count is None or (error_count.dtype is i32 and error_count.get_device() == at))
+    ):
+        _refuse_mrope(q_proj, k_proj, v_proj, positions, sections, rope_cos, rope_sin, slot_mapping, key_cache,
+                      value_cache, num_heads, q_out, inv_rms, q_norm_weight, k_norm_weight, error_count)
+    if q_out is None:
+        q_out = torch.empty((tokens, num_heads, dim), dtype=dtype, device=q_proj.device)
+    one = tokens <= 1  # a stride of one row says nothing
+    packed = _MROPE.pack(
+        q_proj.data_ptr(), k_proj.data_ptr(), v_proj.data_ptr(), 0 if inv_rms is None else inv_rms.data_ptr(),
+        0 if q_norm_weight is None else q_norm_weight.data_ptr(),
+        0 if k_norm_weight is None else k_norm_weight.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(),
+        positions.data_ptr(), 0 if slot_mapping is None else slot_mapping.data_ptr(), q_out.data_ptr(),
+        key_cache.data_ptr(), value_cache.data_ptr(), 0 if error_count is None else error_count.data_ptr(),
+        num_heads * dim if one else qs[0], hkv * dim if one else ks[0], hkv * dim if one else vs[0],
+        kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], tokens, num_heads, hkv, dim, bs, nblk, rope[0],
+        _OUT_DTYPES[proj], _OUT_DTYPES[dtype], axes, 1 if interleaved else 0, *sections, *_NO_SECTIONS[axes:], eps)
+    _launch("simpler_hip_qk_norm_mrope_append", packed, q_proj.device, stream)
+    return q_out
+
+
+_NO_SECTIONS = (0, 0, 0, 0)
+
+
+def _vector(t: torch.Tensor, n: int, at: int) -> bool:
+    return t.dtype is torch.float32 and t.numel() == n and t.is_contiguous() and t.get_device() == at
+
+
+def _refuse_mrope(q_proj, k_proj, v_proj, positions, sections, rope_cos, rope_sin, slot_mapping, key_cache, value_cache,
+                  num_heads, q_out, inv_rms, q_norm_weight, k_norm_weight, error_count) -> None:
+    """Say what is wrong with the arguments of ``qk_norm_mrope_append``."""
+    tokens, dim, dtype, proj, axes = q_proj.shape[0], key_cache.shape[-1], key_cache.dtype, q_proj.dtype, len(sections)
+    if slot_mapping is None and (key_cache.dim() != 3 or key_cache.shape[0] != tokens):
+        raise ValueError("without slot_mapping, key_cache and value_cache are rows [num_tokens, kv_heads, head_dim]")
+    if slot_mapping is not None and key_cache.dim() != 4:
+        raise ValueError("key_cache and value_cache must be [num_blocks, block_size, kv_heads, head_dim]")
+    if dtype not in _HALVES or proj not in _OUT_DTYPES:
         raise ValueError(f"caches must be bfloat16 or float16 and projections also or float32, got {dtype}, {proj}")
-    if value_cache.shape != key_cache.shape or not unit:
+    if value_cache.shape != key_cache.shape or value_cache.dtype is not dtype or key_cache.stride(-1) != 1 \
+            or value_cache.stride(-1) != 1:
         raise ValueError("value_cache must match key_cache, both with unit head-dim stride")
     if not 1 <= axes <= 4 or sum(sections) * 2 != dim:
         raise ValueError(f"sections must be one to four counts that sum to head_dim / 2 = {dim // 2}, got {sections}")
+    hkv = key_cache.shape[-2]
     for t, n, w in ((q_proj, "q_proj", num_heads * dim), (k_proj, "k_proj", hkv * dim), (v_proj, "v_proj", hkv * dim)):
-        if t.dtype is not proj or not t.is_cuda or t.shape != (tokens, w) or t.stride(1) != 1:
-            raise ValueError(f"{n} must be a device {proj} [{tokens}, {w}] tensor with unit stride in its rows")
-    if positions.dtype is not i32 or not positions.is_cuda or positions.shape != (axes, tokens) \
-            or not positions.is_contiguous():
-        raise ValueError(f"positions must be a contiguous int32 device tensor [{axes}, {tokens}]")
+        if t.dtype is not proj or t.shape != (tokens, w) or t.stride(1) != 1:
+            raise ValueError(f"{n} must be a {proj} [{tokens}, {w}] tensor with unit stride in its rows")
     if rope_cos.dim() != 2 or rope_cos.shape[1] != dim or rope_sin.shape != rope_cos.shape:
         raise ValueError("rope tables must be [max_position, head_dim]")
-    small = [(rope_cos, "rope_cos", rope_cos.numel()), (rope_sin, "rope_sin", rope_cos.numel())]
-    small += [(t, n, k) for t, n, k in ((inv_rms, "inv_rms", tokens), (q_norm_weight, "q_norm_weight", dim),
-                                        (k_norm_weight, "k_norm_weight", dim)) if t is not None]
-    for t, n, k in small:
-        if t.dtype is not f32 or not t.is_cuda or not t.is_contiguous() or t.numel() != k:
-            raise ValueError(f"{n} must be a contiguous float32 device tensor of {k} elements")
-    if slot_mapping is not None and (slot_mapping.dtype is not i32 or not slot_mapping.is_cuda
-                                     or slot_mapping.shape != (tokens,) or not slot_mapping.is_contiguous()):
-        raise ValueError("slot_mapping must be a contiguous int32 device tensor [num_tokens]")
-    if error_count is not None and (error_count.dtype is not i32 or not error_count.is_cuda):
-        raise ValueError("error_count must be an int32 device tensor")
-    if not key_cache.is_cuda or not value_cache.is_cuda or value_cache.dtype is not dtype:
-        raise ValueError("key_cache and value_cache must be device tensors of one dtype")
-    if q_out is None:
-        q_out = torch.empty((tokens, num_heads, dim), dtype=dtype, device=q_proj.device)
-    elif q_out.dtype is not dtype or not q_out.is_cuda or not q_out.is_contiguous() or q_out.shape != (tokens, num_heads, dim):
-        raise ValueError(f"q_out must be a contiguous device {dtype} tensor [{tokens}, {num_heads}, {dim}]")
-    if not _one_device(q_proj, k_proj, v_proj, positions, rope_cos, rope_sin, key_cache, value_cache, q_out,
-                       *(t for t in (slot_mapping, inv_rms, q_norm_weight, k_norm_weight) if t is not None)):
-        raise ValueError("the tensors must be on one device")
-    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    row = lambda t: t.stride(0) if tokens > 1 else t.shape[1]  # noqa: E731
-    packed = _MROPE.pack(
-        q_proj.data_ptr(), k_proj.data_ptr(), v_proj.data_ptr(), ptr(inv_rms), ptr(q_norm_weight), ptr(k_norm_weight),
-        rope_cos.data_ptr(), rope_sin.data_ptr(), positions.data_ptr(), ptr(slot_mapping), q_out.data_ptr(),
-        key_cache.data_ptr(), value_cache.data_ptr(), ptr(error_count), row(q_proj), row(k_proj), row(v_proj),
-        *kst, *vst, tokens, num_heads, hkv, dim, bs, nblk, rope_cos.shape[0], _OUT_DTYPES[proj], _OUT_DTYPES[dtype],
-        axes, 1 if interleaved else 0, *sections, *([0] * (4 - axes)), eps)
-    a = _lib.QkNormMropeArgs.from_buffer_copy(packed.ljust(ctypes.sizeof(_lib.QkNormMropeArgs), b"\0"))
-    _launch("simpler_hip_qk_norm_mrope_append", a, q_proj.device, stream)
-    return q_out
+    for t, n, dt, shape in ((positions, "positions", torch.int32, (axes, tokens)),
+                            (slot_mapping, "slot_mapping", torch.int32, (tokens,)),
+                            (rope_cos, "rope_cos", torch.float32, rope_cos.shape),
+                            (rope_sin, "rope_sin", torch.float32, rope_cos.shape), (inv_rms, "inv_rms", torch.float32, None),
+                            (q_norm_weight, "q_norm_weight", torch.float32, (dim,)),
+                            (k_norm_weight, "k_norm_weight", torch.float32, (dim,)),
+                            (q_out, "q_out", dtype, (tokens, num_heads, dim)),
+                            (error_count, "error_count", torch.int32, None)):
+        if t is not None and (t.dtype is not dt or not t.is_contiguous() or (shape is not None and t.shape != shape)):
+            raise ValueError(f"{n} must be a contiguous {dt} tensor{'' if shape is None else f' {list(shape)}'}")
+    if inv_rms is not None and inv_rms.numel() != tokens:
+        raise ValueError(f"inv_rms must have {tokens} elements")
+    raise ValueError("the tensors must be on one device")
 
 
 # ---------------------------------------------------------------------------
@@ -547,25 +580,34 @@ class StepSlots(NamedTuple):
     free_count: torch.Tensor  # [1]
 
 
-_RELEASE, _ASSIGN = struct.Struct("@8P4i"), struct.Struct("@13P5i")
+# SimplerHipReleaseBlocksArgs and SimplerHipAssignSlotsArgs as _lib lays them out
+_RELEASE, _ASSIGN = struct.Struct("@8P4i"), struct.Struct("@13P6i")
+assert _RELEASE.size == ctypes.sizeof(_lib.ReleaseBlocksArgs) and _ASSIGN.size == ctypes.sizeof(_lib.AssignSlotsArgs)
 
 
-def _int32(t: torch.Tensor, name: str, shape: tuple[int, ...], at: int) -> int:
-    """Address of a contiguous int32 tensor of this shape on device ``at``."""
-    if t.dtype is not torch.int32 or not t.is_cuda or t.shape != shape or not t.is_contiguous() or t.get_device() != at:
-        raise ValueError(f"{name} must be a contiguous int32 tensor {list(shape)} on the block table's device, got "
-                         f"{t.dtype} {list(t.shape)} on {t.device}")
-    return t.data_ptr()
-
-
-def _parts(sizes: tuple[int, ...], device: torch.device) -> list[torch.Tensor]:
-    """int32 tensors of these sizes in one allocation, each 16-byte aligned."""
-    starts, at = [], 0
-    for n in sizes:
-        starts.append(at)
-        at += (n + 3) // 4 * 4
-    buf = torch.empty(at, dtype=torch.int32, device=device)
-    return [buf.narrow(0, s, n) for s, n in zip(starts, sizes)]
+def _step_inputs(per_request, name, context_lens, block_table, free_blocks, free_count, error_count) -> tuple[int, ...]:
+    """Addresses of a step's input tensors (and of ``error_count``, or 0), checked."""
+    batch, width = block_table.shape
+    i32, at = torch.int32, block_table.get_device()
+    if not (
+        block_table.dtype is i32 and block_table.is_cuda and block_table.is_contiguous() and per_request.dtype is i32
+        and per_request.shape == (batch,) and per_request.is_contiguous() and per_request.get_device() == at
+        and context_lens.dtype is i32 and context_lens.shape == (batch,) and context_lens.is_contiguous()
+        and context_lens.get_device() == at and free_blocks.dtype is i32 and free_blocks.dim() == 1
+        and free_blocks.is_contiguous() and free_blocks.get_device() == at and free_count.dtype is i32
+        and free_count.shape == (1,) and free_count.get_device() == at
+        and (error_count is None or (error_count.dtype is i32 and error_count.shape == (1,)
+                                     and error_count.get_device() == at))
+    ):
+        for t, n, shape in ((block_table, "block_table", (batch, width)), (per_request, name, (batch,)),
+                            (context_lens, "context_lens", (batch,)), (free_blocks, "free_blocks", free_blocks.shape[:1]),
+                            (free_count, "free_count", (1,)), (error_count, "error_count", (1,))):
+            if t is not None and (t.dtype is not i32 or not t.is_cuda or t.shape != shape or not t.is_contiguous()):
+                raise ValueError(f"{n} must be a contiguous int32 device tensor {list(shape)}, got {t.dtype} "
+                                 f"{list(t.shape)} on {t.device}")
+        raise ValueError("the tensors must be on one device")
+    return (per_request.data_ptr(), context_lens.data_ptr(), block_table.data_ptr(), free_blocks.data_ptr(),
+            free_count.data_ptr(), 0 if error_count is None else error_count.data_ptr())
 
 
 def release_blocks(ended: torch.Tensor, context_lens: torch.Tensor, block_table: torch.Tensor,
@@ -580,15 +622,12 @@ def release_blocks(ended: torch.Tensor, context_lens: torch.Tensor, block_table:
     For requests that own their blocks alone: ids that two rows share would be
     returned twice. Everything int32 and contiguous; at most 4096 requests.
     """
-    (batch, width), device, at = block_table.shape, block_table.device, block_table.get_device()
-    inputs = (_int32(ended, "ended", (batch,), at), _int32(context_lens, "context_lens", (batch,), at),
-              _int32(block_table, "block_table", (batch, width), at),
-              _int32(free_blocks, "free_blocks", free_blocks.shape[:1], at), _int32(free_count, "free_count", (1,), at))
-    errors = 0 if error_count is None else _int32(error_count, "error_count", (1,), at)
-    lens_out, count_out = _parts((batch, 1), device)
-    a = _lib.ReleaseBlocksArgs.from_buffer_copy(_RELEASE.pack(
-        *inputs, lens_out.data_ptr(), count_out.data_ptr(), errors, batch, width, block_size, free_blocks.shape[0]))
-    _launch("simpler_hip_release_blocks", a, device, stream)
+    *inputs, errors = _step_inputs(ended, "ended", context_lens, block_table, free_blocks, free_count, error_count)
+    (batch, width), device = block_table.shape, block_table.device
+    count_out, lens_out = torch.empty(batch + 1, dtype=torch.int32, device=device).split_with_sizes((1, batch))
+    at = count_out.data_ptr()
+    _launch("simpler_hip_release_blocks", _RELEASE.pack(*inputs, at + 4, at, errors, batch, width, block_size,
+                                                        free_blocks.shape[0]), device, stream)
     return ReleasedBlocks(lens_out, count_out)
 
 
@@ -612,15 +651,13 @@ def assign_slots(new_lens: torch.Tensor, context_lens: torch.Tensor, block_table
     """
     if num_tokens < 0:
         raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
-    (batch, width), device, at = block_table.shape, block_table.device, block_table.get_device()
-    inputs = (_int32(new_lens, "new_lens", (batch,), at), _int32(context_lens, "context_lens", (batch,), at),
-              _int32(block_table, "block_table", (batch, width), at),
-              _int32(free_blocks, "free_blocks", free_blocks.shape[:1], at), _int32(free_count, "free_count", (1,), at))
-    errors = 0 if error_count is None else _int32(error_count, "error_count", (1,), at)
-    parts = _parts(
-        (num_tokens, num_tokens, num_tokens, batch + 1, batch, batch, 1), device)
-    a = _lib.AssignSlotsArgs.from_buffer_copy(_ASSIGN.pack(
-        *inputs, *(t.data_ptr() for t in parts), errors, batch, width, block_size, free_blocks.shape[0],
-        num_tokens).ljust(ctypes.sizeof(_lib.AssignSlotsArgs), b"\0"))
-    _launch("simpler_hip_assign_slots", a, device, stream)
+    *inputs, errors = _step_inputs(new_lens, "new_lens", context_lens, block_table, free_blocks, free_count, error_count)
+    (batch, width), device, n = block_table.shape, block_table.device, num_tokens
+    buf = torch.empty(3 * n + 3 * batch + 2, dtype=torch.int32, device=device)
+    parts = buf.split_with_sizes((n, n, n, batch + 1, batch, batch, 1))
+    at, b4, n4 = buf.data_ptr(), 4 * batch, 4 * n
+    after = at + 3 * n4
+    _launch("simpler_hip_assign_slots", _ASSIGN.pack(
+        *inputs, at, at + n4, at + 2 * n4, after, after + b4 + 4, after + 2 * b4 + 4, after + 3 * b4 + 4, errors, batch,
+        width, block_size, free_blocks.shape[0], n, 0), device, stream)
     return StepSlots(*parts)
