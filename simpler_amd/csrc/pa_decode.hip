@@ -125,14 +125,18 @@ struct Kernels {
     MergeFn merge;
 };
 
-KernelPair pick_int4(int d, int groups, int out) {
-    return d == 64 ? pick_int4_d64(groups, out) : d == 128 ? pick_int4_d128(groups, out)
-         : d == 256 ? pick_int4_d256(groups, out) : KernelPair{};
+KernelPair pick_int4(int d, int groups, int rows, int out) {
+    return d == 64    ? pick_int4_d64(groups, rows, out)
+           : d == 128 ? pick_int4_d128(groups, rows, out)
+           : d == 256 ? pick_int4_d256(groups, rows, out)
+                      : KernelPair{};
 }
 
-DirectFn pick_int4_direct(int d, int groups, int out) {
-    return d == 64 ? pick_int4_direct_d64(groups, out) : d == 128 ? pick_int4_direct_d128(groups, out)
-         : d == 256 ? pick_int4_direct_d256(groups, out) : DirectFn{};
+DirectFn pick_int4_direct(int d, int groups, int rows, int out) {
+    return d == 64    ? pick_int4_direct_d64(groups, rows, out)
+           : d == 128 ? pick_int4_direct_d128(groups, rows, out)
+           : d == 256 ? pick_int4_direct_d256(groups, rows, out)
+                      : DirectFn{};
 }
 
 Kernels pick_kernel(const SimplerHipPaDecodeArgs *a, bool append = false) {
@@ -146,8 +150,10 @@ Kernels pick_kernel(const SimplerHipPaDecodeArgs *a, bool append = false) {
         }
     } else if (is_int4(a)) {
         if (!append && (a->kv_group == 32 || a->kv_group == 64 || a->kv_group == 128)) {  // no fused append
-            s.k = pick_int4(dk, dk / a->kv_group, out);
-            s.direct = pick_int4_direct(dk, dk / a->kv_group, out);
+            const int64_t rows = (int64_t)(a->num_heads / a->num_kv_heads) * a->q_len;
+            const int few = (int)std::min<int64_t>(rows, 16);
+            s.k = pick_int4(dk, dk / a->kv_group, few, out);
+            s.direct = pick_int4_direct(dk, dk / a->kv_group, few, out);
         }
     } else if (is_mla_shape(a)) {
         // (the kernel's fill offsets use 24-bit multiplies: token rows below 8 MB)
@@ -308,9 +314,13 @@ Plan make_plan(const SimplerHipPaDecodeArgs *a, const KernelPair &k) {  // k: th
         // Row tiles of one kv head run as sibling waves of one worker workgroup
         // (up to four), so K/V of a block is fetched once for all of them;
         // two row tiles with K through LDS run in one wave instead.
-        // 4-bit caches: pairs of row tiles, without siblings.
+        // 4-bit caches: without siblings; from three row tiles on they go in
+        // pairs, whose wave turns K's and V's codes into fragments once for
+        // both (13 to 16 sequences of up to 9000 tokens, 8 kv heads of 128 dims,
+        // 4 row tiles 72 us against 81, 3 tiles 69 against 70.3; 2 tiles are
+        // faster alone, 46.6 us against 50.7: the pair's wave spills).
         const bool int4 = is_int4(a);
-        const bool pair = k.main_pair && (int4 ? p.row_tiles >= 2 : p.row_tiles == 2);
+        const bool pair = k.main_pair && (int4 ? p.row_tiles > 2 : p.row_tiles == 2);
         p.tiles_per_worker = pair ? 2 : int4 ? 1 : (p.row_tiles < kMaxWavesPerWorker ? p.row_tiles : kMaxWavesPerWorker);
         p.threads = pair ? 64 : 64 * p.tiles_per_worker;
         p.main = pair ? k.main_pair : p.tiles_per_worker > 1 ? k.main_multi : k.main;
@@ -359,6 +369,31 @@ Plan make_plan(const SimplerHipPaDecodeArgs *a, const KernelPair &k) {  // k: th
     return p;
 }
 
+// 4-bit caches: a wave takes about 2.1 us per 64-token chunk (3.2 above 128
+// dims) and the direct kernel 6 us besides, the lists and their merge 6 to 7 us
+// more, three chunks' time. So the direct kernel is taken where a wave's chunks
+// are at most three more than a list worker's, were every sequence as long as
+// the table allows; and at most 8, as one long sequence among short ones keeps
+// only its own waves busy (16 us, against 14). A workgroup takes as many waves
+// as leave the tiles resident together, 2048 waves. Measured, direct / lists in
+// us, 8 kv heads of 128 dims, 4 heads each, as sequences x tokens:
+//   8 x 128 7.5 / 13.5, x 1024 11.3 / 14.7, x 2048 15.8 / 16.5 (x 4096 24.0 / 20.6);
+//   32 x 512 10.0 / 17.2, x 2048 17.4 / 24.9, x 4096 30.3 / 36.3;
+//   128 x 512 18.0 / 26.3 (with 8 waves 34.5), x 1024 30.5 / 37.3;
+//   200 x 512, 8 heads each, 28.2 / 36.6 with one wave, 32.1 with four.
+int int4_direct_waves(const SimplerHipPaDecodeArgs *a, const Kernels &s, const Plan &p) {
+    constexpr int64_t kWaves = 2048, kMaxSteps = 8, kMoreSteps = 3;
+    const int64_t chunks = ((int64_t)a->max_blocks_per_seq * a->block_size + 63) / 64;
+    const int64_t tiles = std::max<int64_t>((int64_t)a->batch * a->num_kv_heads * p.row_tiles, 1);
+    int64_t waves = 1;
+    while (2 * waves * tiles <= kWaves && 2 * waves <= s.direct.max_waves) waves *= 2;
+    waves = std::max<int64_t>(std::min(waves, chunks), 1);
+    const int64_t steps = (chunks + waves - 1) / waves;
+    if (steps > kMaxSteps || (steps - kMoreSteps) * kWaves > tiles * chunks) return 0;
+    if (tiles > 1 << 24) return 0;  // a launch's threads count to 2^32
+    return (int)waves;
+}
+
 // Waves per workgroup of the short-context kernels (pa_kernels_direct.h), or 0
 // where the work lists run: the caller forced a worker count, or a context may
 // be long (the host knows the table's width, not the lengths). One workgroup
@@ -391,14 +426,6 @@ Plan make_plan(const SimplerHipPaDecodeArgs *a, const KernelPair &k) {  // k: th
 //   174 / 127; 15 x 8 of 380 tokens, 64 rows of 128 dims, 90 MB, 23.5 / 20.9).
 //   Above 64 dims, 768 KB over the row tiles of a kv head at most.
 // Waves per tile: enough for workers_per_cu waves on every CU, at least four.
-int int4_direct_waves(const SimplerHipPaDecodeArgs *a, const Kernels &s, const Plan &p) {
-    const int64_t tokens = (int64_t)a->max_blocks_per_seq * a->block_size;
-    const int64_t chunks = (tokens + 63) / 64;
-    const int64_t waves = std::min<int64_t>(s.direct.max_waves, chunks);
-    if ((chunks + waves - 1) / waves > 2) return 0;
-    return (int)waves;
-}
-
 int direct_waves(const SimplerHipPaDecodeArgs *a, const Kernels &s, const Plan &p) {
     if (!s.direct.fn || a->num_workers > 0) return 0;
     if (is_int4(a)) return int4_direct_waves(a, s, p);

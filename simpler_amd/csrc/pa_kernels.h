@@ -2680,14 +2680,14 @@ DirectFn pick_direct_bf16(int bs, int d, int out_dtype);
 DirectFn pick_direct_f16(int bs, int d, int out_dtype);
 DirectFn pick_direct_fp8(int bs, int d, int out_dtype);
 // GQA decode with 4-bit caches (pa_kernels_int4.h), Dk == Dv, `groups`
-// scales per row, bf16 or fp16 query: main and main_pair run one and two row
-// tiles per wave.
-KernelPair pick_int4_d64(int groups, int out_dtype);
-KernelPair pick_int4_d128(int groups, int out_dtype);
-KernelPair pick_int4_d256(int groups, int out_dtype);
-DirectFn pick_int4_direct_d64(int groups, int out_dtype);
-DirectFn pick_int4_direct_d128(int groups, int out_dtype);
-DirectFn pick_int4_direct_d256(int groups, int out_dtype);
+// scales per row, `rows` query rows per kv head, bf16 or fp16 query: main and
+// main_pair run one and two row tiles per wave.
+KernelPair pick_int4_d64(int groups, int rows, int out_dtype);
+KernelPair pick_int4_d128(int groups, int rows, int out_dtype);
+KernelPair pick_int4_d256(int groups, int rows, int out_dtype);
+DirectFn pick_int4_direct_d64(int groups, int rows, int out_dtype);
+DirectFn pick_int4_direct_d128(int groups, int rows, int out_dtype);
+DirectFn pick_int4_direct_d256(int groups, int rows, int out_dtype);
 // MLA (Dk 576, Dv 512, V a prefix of K), bf16.
 KernelPair pick_mla(int bs, int out_dtype);
 // The split merge for output width dv.

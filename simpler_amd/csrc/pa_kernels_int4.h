@@ -31,6 +31,12 @@
 // pc = lane % 16 and tokens 4 qd + e (qd = lane / 16) of each tile, which is the
 // A operand of P V over two tiles. The pages' order of nibbles is the operands'
 // own: a lane loads D/8 consecutive bytes per tile for K and for V.
+// Few rows. Up to 8 (4) query rows per kv head would leave half (three quarters)
+// of the score lanes without a row. There lane pc takes row pc % (16 / C) of
+// token tile pc / (16 / C) out of every C tiles (C = 2, 4): Q is in all the
+// columns, a lane keeps its own tile's products, and the softmax runs on 64 / C
+// tokens' worth of registers per chunk. In P V a lane's operand is zero where the
+// k-steps are another tile's, so the C copies of a row add up to it at the end.
 // Scales: lane i loads token i's, the wave shares them through LDS.
 // K(i+1) is loaded into K(i)'s registers right after QK(i), V(i+1) after PV(i).
 #pragma once
@@ -49,8 +55,8 @@ __device__ __forceinline__ u32x4_t nibbles_subnormal(const unsigned x) {
 
 // The same pairs as fp16 integers c - 8, exact: 1024 + c - 1032 and
 // (1024 + 16 c) / 16 - 72. The masks and the 1024s come in registers (`low`,
-// `high`, `k1024`), for one v_and_or_b32 per pair: as literals
-// they take an and and an or.
+// `high`, `k1024`), for one v_and_or_b32 per pair: as literals they take an and
+// and an or.
 __device__ __forceinline__ u32x4_t nibbles_centred(const unsigned x, const unsigned low, const unsigned high,
                                                    const unsigned k1024) {
     const f16x2_t off = (f16x2_t){(_Float16)-1032.f, (_Float16)-1032.f};
@@ -95,7 +101,7 @@ __device__ __forceinline__ void int4_store2(void *out, const int64_t off, const 
 // of the row tiles rt .. rt + RTW - 1 of (b, kvh): the final output where they
 // are the whole tile, else a piece each (see finish_segment). D: head dim, NG:
 // groups per row. `lds`: this wave's int4_wave_lds bytes.
-template <int D, int NG, int RTW, bool EXACT>
+template <int D, int NG, int RTW, int C, bool EXACT>
 __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const int b, const int kvh, const int rt,
                                                  const int ctx, const int seg_begin, const int seg_end,
                                                  const bool whole, float *const part_o, float *const part_ml,
@@ -106,13 +112,14 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
     constexpr int GT = DT / NG;   // dim tiles per group
     constexpr int LW = D / 32;    // words of codes per lane and tile
     constexpr int DH = D / 64;    // words per lane, tile and token pair of V
-    // Where registers are short the tiles' work is kept apart: the scheduler
-    // would otherwise mix it and spill.
-    constexpr bool kTight = true;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
     constexpr float kSlack = 8.f;  // a score may pass the frame by 2^kSlack
+    constexpr int R16 = 16 / C;   // rows of a tile
+    constexpr int NS = 4 / C;     // sets of C token tiles
     static_assert(D % 64 == 0 && KS % NG == 0, "head dims: multiples of 64, groups of whole k-steps");
+    static_assert(C == 1 || RTW == 1, "several row tiles: 16 rows each");
     const int lane = threadIdx.x & 63, qd = lane >> 4, pc = lane & 15;
+    const int tq = pc / R16, pr = pc % R16;  // this lane's token tile of a set, its row
     const int bs = P.block_size, sh = __builtin_ctz(bs);
     const bool f16 = P.half16;
     // constants of the conversions, kept in registers
@@ -121,89 +128,22 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
     asm volatile("" : "+v"(k1024));
     auto centred = [&](const unsigned x) { return nibbles_centred(x, low, high, k1024); };
 
-    // ---- Q: row pc of each row tile, in the codes' nibble order, exponent-aligned ----
-    u32x4_t qv[RTW][KS];
-    float zq[RTW][NG];  // sum of the group's q, in the units of the scores
-    float xs[RTW];      // scores to log2 units
-    int rowlim[RTW];    // first token the row does not see (within the segment's end)
+    // ---- the query's rows ----
+    u32x4_t raw[RTW][KS];
+    int rowlim[RTW];  // first token the row does not see (within the segment's end)
 #pragma unroll
     for (int r = 0; r < RTW; ++r) {
         rowlim[r] = 0;
-        u32x4_t raw[KS];
 #pragma unroll
-        for (int j = 0; j < KS; ++j) raw[j] = (u32x4_t){0u, 0u, 0u, 0u};
-        if (pc < min(16, P.rows - (rt + r) * 16)) {
-            const int row = (rt + r) * 16 + pc, i = row / P.group, hh = row - i * P.group;
+        for (int j = 0; j < KS; ++j) raw[r][j] = (u32x4_t){0u, 0u, 0u, 0u};
+        if (pr < min(16, P.rows - (rt + r) * 16)) {
+            const int row = (rt + r) * 16 + pr, i = row / P.group, hh = row - i * P.group;
             const uint16_t *qrow = P.q + ((int64_t)(b * P.q_len + i) * P.num_heads + kvh * P.group + hh) * D;
 #pragma unroll
-            for (int j = 0; j < KS; ++j) raw[j] = ld16(qrow + 32 * j + 8 * qd);
+            for (int j = 0; j < KS; ++j) raw[r][j] = ld16(qrow + 32 * j + 8 * qd);
             rowlim[r] = min(seg_end, P.causal ? ctx - (P.q_len - 1 - i) : ctx);
         }
-        float f[KS][8], amax = 0.f;
-        if (f16) {
-#pragma unroll
-            for (int j = 0; j < KS; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) f[j][2 * i] = half_lo(raw[j][i]), f[j][2 * i + 1] = half_hi(raw[j][i]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < KS; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    f[j][2 * i] = __uint_as_float(raw[j][i] << 16), f[j][2 * i + 1] = __uint_as_float(raw[j][i] & 0xffff0000u);
-        }
-#pragma unroll
-        for (int j = 0; j < KS; ++j)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[j][i]));
-        amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-        // the row times 2^(140 - eb): its largest element in [2^13, 2^14)
-        const int eb = min(max((int)(__float_as_uint(amax) >> 23), 27), 240);
-        float up = __uint_as_float((unsigned)(267 - eb) << 23);
-        if (P.scale < 0.f) up = -up;  // the scores' sign, so that their maximum is the softmax's
-        const float sub = EXACT ? 1.f : 0.0625f;  // nibbles at bits 4..7: 16 c
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            float s = 0.f;
-#pragma unroll
-            for (int j = g * GM; j < (g + 1) * GM; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s += f[j][i];
-            s += __shfl_xor(s, 16, 64);
-            s += __shfl_xor(s, 32, 64);
-            zq[r][g] = s * up * (EXACT ? 1.f : 0x1p-24f);
-        }
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
-            const float u16 = up * sub;
-            qv[r][j] = (u32x4_t){Elem<_Float16>::pack2(f[j][0] * up, f[j][4] * up),
-                                 Elem<_Float16>::pack2(f[j][1] * u16, f[j][5] * u16),
-                                 Elem<_Float16>::pack2(f[j][2] * up, f[j][6] * up),
-                                 Elem<_Float16>::pack2(f[j][3] * u16, f[j][7] * u16)};
-        }
-        xs[r] = fabsf(P.scale) * kLog2e * __uint_as_float((unsigned)(eb - 13) << 23) * (EXACT ? 1.f : 0x1p24f);
-        xs[r] = fmaxf(xs[r], 0x1p-120f);  // scale 0: masked scores stay -inf (0 times inf is NaN)
     }
-    // tokens before this one are seen by every row of the wave's tiles
-    const int all_see = P.causal ? ctx - (P.q_len - 1 - (rt * 16) / P.group) : ctx;
-
-    f32x4_t acc[RTW][DT];
-    float lsum[RTW], zacc[RTW][NG], fy[RTW], nf[RTW], thr[RTW];
-    int kexp = -64;  // exponent of the frame that the V scales set
-    float slim = 0x1p-58f;
-#pragma unroll
-    for (int r = 0; r < RTW; ++r) {
-#pragma unroll
-        for (int j = 0; j < DT; ++j) acc[r][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int g = 0; g < NG; ++g) zacc[r][g] = 0.f;
-        lsum[r] = 0.f;
-        fy[r] = -INFINITY;
-        nf[r] = 0.f;
-        thr[r] = -INFINITY;
-    }
-
     const __attribute__((address_space(4))) int32_t *bt_row =
         (const __attribute__((address_space(4))) int32_t *)(P.block_table + (int64_t)b * P.max_blocks);
     const char *k_head = reinterpret_cast<const char *>(P.k) + (int64_t)kvh * P.k_head_stride;
@@ -267,6 +207,86 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
             load_codes(vreg[t], v_head + page[t] * P.v_block_stride + row_of(tok0, t) * (D / 2) + v_lane);
     };
 
+    // Everything that the first chunk needs is on its way before the query is
+    // waited for: its rows, then (the block ids are scalar loads) scales, K, V.
+    read_ids(seg_begin);
+    resolve();
+    load_scales(seg_begin);
+    load_k(seg_begin);
+    load_v(seg_begin);
+    read_ids(seg_begin + kInt4Chunk);
+
+    // ---- Q in the codes' nibble order, exponent-aligned ----
+    u32x4_t qv[RTW][KS];
+    float zq[RTW][NG];  // sum of the group's q, in the units of the scores
+    float xs[RTW];      // scores to log2 units
+#pragma unroll
+    for (int r = 0; r < RTW; ++r) {
+        float f[KS][8], amax = 0.f;
+        if (f16) {
+#pragma unroll
+            for (int j = 0; j < KS; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[j][2 * i] = half_lo(raw[r][j][i]), f[j][2 * i + 1] = half_hi(raw[r][j][i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < KS; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    f[j][2 * i] = __uint_as_float(raw[r][j][i] << 16), f[j][2 * i + 1] = __uint_as_float(raw[r][j][i] & 0xffff0000u);
+        }
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[j][i]));
+        amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+        // the row times 2^(140 - eb): its largest element in [2^13, 2^14)
+        const int eb = min(max((int)(__float_as_uint(amax) >> 23), 27), 240);
+        float up = __uint_as_float((unsigned)(267 - eb) << 23);
+        if (P.scale < 0.f) up = -up;  // the scores' sign, so that their maximum is the softmax's
+        const float sub = EXACT ? 1.f : 0.0625f;  // nibbles at bits 4..7: 16 c
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = g * GM; j < (g + 1) * GM; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s += f[j][i];
+            s += __shfl_xor(s, 16, 64);
+            s += __shfl_xor(s, 32, 64);
+            zq[r][g] = s * up * (EXACT ? 1.f : 0x1p-24f);
+        }
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            const float u16 = up * sub;
+            qv[r][j] = (u32x4_t){Elem<_Float16>::pack2(f[j][0] * up, f[j][4] * up),
+                                 Elem<_Float16>::pack2(f[j][1] * u16, f[j][5] * u16),
+                                 Elem<_Float16>::pack2(f[j][2] * up, f[j][6] * up),
+                                 Elem<_Float16>::pack2(f[j][3] * u16, f[j][7] * u16)};
+        }
+        xs[r] = fabsf(P.scale) * kLog2e * __uint_as_float((unsigned)(eb - 13) << 23) * (EXACT ? 1.f : 0x1p24f);
+        xs[r] = fmaxf(xs[r], 0x1p-120f);  // scale 0: masked scores stay -inf (0 times inf is NaN)
+    }
+    // tokens before this one are seen by every row of the wave's tiles
+    const int all_see = P.causal ? ctx - (P.q_len - 1 - (rt * 16) / P.group) : ctx;
+
+    f32x4_t acc[RTW][DT];
+    float lsum[RTW], zacc[RTW][NG], fy[RTW], nf[RTW], thr[RTW];
+    int kexp = -64;  // exponent of the frame that the V scales set
+    float slim = 0x1p-58f;
+#pragma unroll
+    for (int r = 0; r < RTW; ++r) {
+#pragma unroll
+        for (int j = 0; j < DT; ++j) acc[r][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int g = 0; g < NG; ++g) zacc[r][g] = 0.f;
+        lsum[r] = 0.f;
+        fy[r] = -INFINITY;
+        nf[r] = 0.f;
+        thr[r] = -INFINITY;
+    }
+
     unsigned *const kst = reinterpret_cast<unsigned *>(lds);  // [g][token]: s, z (EXACT: fp32 s, z + 8 s)
     unsigned *const vst = kst + NG * kInt4Chunk * (EXACT ? 2 : 1);
     bool first = true;
@@ -310,61 +330,72 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
             read_ids(tok0 + 2 * kInt4Chunk);
         }
         wave_lds_sync();
-        // scale and zero of tile t's tokens 4qd .. 4qd+3
-        auto scales_of = [&](const unsigned *st, const int g, const int t, f32x4_t &s, f32x4_t &z) {
+        // scale and zero of tokens 4qd .. 4qd+3 of this lane's tile of set u
+        auto scales_of = [&](const unsigned *st, const int g, const int u, f32x4_t &s, f32x4_t &z) {
+            const int at = g * kInt4Chunk + 16 * C * u + 16 * tq + 4 * qd;
             if constexpr (EXACT) {
-                const f32x4_t *p = reinterpret_cast<const f32x4_t *>(st) + (g * kInt4Chunk + 16 * t + 4 * qd) / 2;
+                const f32x4_t *p = reinterpret_cast<const f32x4_t *>(st) + at / 2;
                 const f32x4_t a = p[0], c = p[1];
                 s = (f32x4_t){a[0], a[2], c[0], c[2]};
                 z = (f32x4_t){a[1], a[3], c[1], c[3]};
             } else {
-                const u32x4_t w = *reinterpret_cast<const u32x4_t *>(st + g * kInt4Chunk + 16 * t + 4 * qd);
+                const u32x4_t w = *reinterpret_cast<const u32x4_t *>(st + at);
                 s = (f32x4_t){half_lo(w[0]), half_lo(w[1]), half_lo(w[2]), half_lo(w[3])};
                 z = (f32x4_t){half_hi(w[0]), half_hi(w[1]), half_hi(w[2]), half_hi(w[3])};
             }
         };
 
         // ---- scores ----
-        f32x4_t y[RTW][4];
+        f32x4_t y[RTW][NS];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int u = 0; u < NS; ++u) {
+            f32x4_t own[RTW][NG];  // q . c of this lane's tile
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                f32x4_t dot[RTW];
+            for (int i = 0; i < C; ++i) {
 #pragma unroll
-                for (int j = g * GM; j < (g + 1) * GM; ++j) {
-                    const u32x4_t a = EXACT ? centred(kreg[t][j]) : nibbles_subnormal(kreg[t][j]);
+                for (int g = 0; g < NG; ++g) {
+                    f32x4_t dot[RTW];
+#pragma unroll
+                    for (int j = g * GM; j < (g + 1) * GM; ++j) {
+                        const u32x4_t a = EXACT ? centred(kreg[u * C + i][j]) : nibbles_subnormal(kreg[u * C + i][j]);
+#pragma unroll
+                        for (int r = 0; r < RTW; ++r)
+                            dot[r] = Elem<_Float16>::mma32(a, qv[r][j],
+                                                           j == g * GM ? (f32x4_t){0.f, 0.f, 0.f, 0.f} : dot[r]);
+                    }
 #pragma unroll
                     for (int r = 0; r < RTW; ++r)
-                        dot[r] = Elem<_Float16>::mma32(a, qv[r][j],
-                                                       j == g * GM ? (f32x4_t){0.f, 0.f, 0.f, 0.f} : dot[r]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) own[r][g][e] = i == 0 || tq == i ? dot[r][e] : own[r][g][e];
                 }
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
                 f32x4_t s, z;
-                scales_of(kst, g, t, s, z);
+                scales_of(kst, g, u, s, z);
 #pragma unroll
                 for (int r = 0; r < RTW; ++r)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         // (adding 0 in a fused form takes fp16 operands as they are)
-                        const float zz = __builtin_fmaf(z[e], zq[r][g], g == 0 ? 0.f : y[r][t][e]);
-                        y[r][t][e] = __builtin_fmaf(s[e], dot[r][e], zz);
+                        const float zz = __builtin_fmaf(z[e], zq[r][g], g == 0 ? 0.f : y[r][u][e]);
+                        y[r][u][e] = __builtin_fmaf(s[e], own[r][g][e], zz);
                     }
             }
-            if constexpr (kTight) __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
         if constexpr (NEXT) load_k(tok0 + kInt4Chunk);
-        __builtin_amdgcn_sched_barrier(0);
 
         // ---- frame ----
         if (tok0 + kInt4Chunk > min(seg_end, all_see) || bad_now) {  // some row does not see some token
 #pragma unroll
-            for (int r = 0; r < RTW; ++r)
+            for (int u = 0; u < NS; ++u) {
+                const int t = C * u + tq;
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
+                for (int r = 0; r < RTW; ++r)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (tok0 + 16 * t + 4 * qd + e >= rowlim[r] || ((bad_now >> t) & 1)) y[r][t][e] = -INFINITY;
+                        if (tok0 + 16 * t + 4 * qd + e >= rowlim[r] || ((bad_now >> t) & 1)) y[r][u][e] = -INFINITY;
+            }
         }
         float ymax[RTW];
         bool move = first || smax > slim;
@@ -372,10 +403,9 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
         for (int r = 0; r < RTW; ++r) {
             ymax[r] = -INFINITY;
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int u = 0; u < NS; ++u)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    ymax[r] = fmaxf(ymax[r], y[r][t][e]);
+                for (int e = 0; e < 4; ++e) ymax[r] = fmaxf(ymax[r], y[r][u][e]);
             move |= ymax[r] > thr[r];
         }
         if (__any(move)) {
@@ -391,6 +421,8 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
             for (int r = 0; r < RTW; ++r) {
                 float m = fmaxf(ymax[r], __shfl_xor(ymax[r], 16, 64));
                 m = fmaxf(m, __shfl_xor(m, 32, 64));
+                if constexpr (C >= 2) m = fmaxf(m, __shfl_xor(m, 8, 64));
+                if constexpr (C >= 4) m = fmaxf(m, __shfl_xor(m, 4, 64));
                 m = fmaxf(m, fy[r]);
                 const float a =
                     (fy[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((fy[r] - m) * xs[r])) * kdown;
@@ -410,41 +442,64 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
         }
 
         // ---- p, its sums, and P V: two tiles at a time ----
+        f32x4_t p[RTW][2];  // of the sets in hand
+        u32x2_t ps[RTW][NG][2], pl[RTW][NG][2];  // p s, the A operands (EXACT: and what its rounding left)
+        auto weights = [&](const int i, const int u) {
+#pragma unroll
+            for (int r = 0; r < RTW; ++r) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    p[r][i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[r][u][e], xs[r], nf[r]));
+                lsum[r] += (p[r][i][0] + p[r][i][1]) + (p[r][i][2] + p[r][i][3]);
+            }
+        };
+        auto scaled = [&](const int i, const int u, const int g) {
+            f32x4_t s, z;
+            scales_of(vst, g, u, s, z);
+#pragma unroll
+            for (int r = 0; r < RTW; ++r) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = __builtin_fmaf(p[r][i][e], s[e], 0.f);
+                    zacc[r][g] = __builtin_fmaf(p[r][i][e], z[e], zacc[r][g]);
+                }
+                const u32x2_t w = {Elem<_Float16>::pack2(v[0], v[1]), Elem<_Float16>::pack2(v[2], v[3])};
+                ps[r][g][i] = w;
+                if constexpr (EXACT)
+                    pl[r][g][i] = (u32x2_t){Elem<_Float16>::pack2(v[0] - half_lo(w[0]), v[1] - half_hi(w[0])),
+                                            Elem<_Float16>::pack2(v[2] - half_lo(w[1]), v[3] - half_hi(w[1]))};
+            }
+        };
 #pragma unroll
         for (int t = 0; t < 4; t += 2) {
-            f32x4_t p[RTW][2];
+            if constexpr (C == 1) {
+                weights(0, t);
+                weights(1, t + 1);
+            } else if (t % C == 0) {
+                weights(0, t / C);
 #pragma unroll
-            for (int r = 0; r < RTW; ++r)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        p[r][i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[r][t + i][e], xs[r], nf[r]));
-                    lsum[r] += (p[r][i][0] + p[r][i][1]) + (p[r][i][2] + p[r][i][3]);
-                }
+                for (int g = 0; g < NG; ++g) scaled(0, t / C, g);
+            }
+            // A's first four k of a lane are tile t's tokens, the others tile t + 1's: with C > 1 a lane has one
+            // of the set's tiles and zeros for the others
+            auto operand = [&](const u32x2_t (&w)[2]) {
+                if constexpr (C == 1) return (u32x4_t){w[0][0], w[0][1], w[1][0], w[1][1]};
+                const bool even = tq == t % C, odd = tq == t % C + 1;
+                return (u32x4_t){even ? w[0][0] : 0u, even ? w[0][1] : 0u, odd ? w[0][0] : 0u, odd ? w[0][1] : 0u};
+            };
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                u32x2_t ps[RTW][2], pl[RTW][2];  // p s, the A operands (EXACT: and what its rounding left)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    f32x4_t s, z;
-                    scales_of(vst, g, t + i, s, z);
-#pragma unroll
-                    for (int r = 0; r < RTW; ++r) {
-                        float v[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            v[e] = __builtin_fmaf(p[r][i][e], s[e], 0.f);
-                            zacc[r][g] = __builtin_fmaf(p[r][i][e], z[e], zacc[r][g]);
-                        }
-                        ps[r][i] = (u32x2_t){Elem<_Float16>::pack2(v[0], v[1]), Elem<_Float16>::pack2(v[2], v[3])};
-                        if constexpr (EXACT)
-                            pl[r][i] = (u32x2_t){
-                                Elem<_Float16>::pack2(v[0] - half_lo(ps[r][i][0]), v[1] - half_hi(ps[r][i][0])),
-                                Elem<_Float16>::pack2(v[2] - half_lo(ps[r][i][1]), v[3] - half_hi(ps[r][i][1]))};
-                    }
+                if constexpr (C == 1) {
+                    scaled(0, t, g);
+                    scaled(1, t + 1, g);
                 }
-                if constexpr (kTight) __builtin_amdgcn_sched_barrier(0);
+                u32x4_t pa[RTW], pb[RTW];
+#pragma unroll
+                for (int r = 0; r < RTW; ++r) {
+                    pa[r] = operand(ps[r][g]);
+                    if constexpr (EXACT) pb[r] = operand(pl[r][g]);
+                }
 #pragma unroll
                 for (int h = 0; h < DH; ++h) {
                     if (4 * h + 3 < g * GT || 4 * h >= (g + 1) * GT) continue;  // no dim tile of this group
@@ -457,33 +512,27 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
                         const u32x4_t vv = (u32x4_t){a[n], c[n], a2[n], c2[n]};
 #pragma unroll
                         for (int r = 0; r < RTW; ++r) {
-                            acc[r][j] = Elem<_Float16>::mma32((u32x4_t){ps[r][0][0], ps[r][0][1], ps[r][1][0], ps[r][1][1]},
-                                                              vv, acc[r][j]);
-                            if constexpr (EXACT)
-                                acc[r][j] = Elem<_Float16>::mma32(
-                                    (u32x4_t){pl[r][0][0], pl[r][0][1], pl[r][1][0], pl[r][1][1]}, vv, acc[r][j]);
+                            acc[r][j] = Elem<_Float16>::mma32(pa[r], vv, acc[r][j]);
+                            if constexpr (EXACT) acc[r][j] = Elem<_Float16>::mma32(pb[r], vv, acc[r][j]);
                         }
                     }
                 }
-                if constexpr (kTight) __builtin_amdgcn_sched_barrier(0);
             }
         }
-        __builtin_amdgcn_sched_barrier(0);
         if constexpr (NEXT) load_v(tok0 + kInt4Chunk);
-        __builtin_amdgcn_sched_barrier(0);
     };
 
-    read_ids(seg_begin);
-    resolve();
-    load_scales(seg_begin);
-    load_k(seg_begin);
-    load_v(seg_begin);
-    read_ids(seg_begin + kInt4Chunk);
     int tok0 = seg_begin;
     for (; tok0 + kInt4Chunk < seg_end; tok0 += kInt4Chunk) step(tok0, std::true_type{});
     step(tok0, std::false_type{});
 
-    // ---- output or pieces: lane holds rows 4qd+e, dims 32u + 2pc, + 1 ----
+    // ---- output or pieces: lane holds rows 4qd+e, dims 32u + 2pc, + 1; with
+    // C > 1 each tile of a set has its own copy of a row, summed here ----
+    auto over_tiles = [&](float x) {  // over the copies in the lanes pc
+        if constexpr (C >= 2) x += __shfl_xor(x, 8, 64);
+        if constexpr (C >= 4) x += __shfl_xor(x, 4, 64);
+        return x;
+    };
 #pragma unroll
     for (int r = 0; r < RTW; ++r) {
         const int rows_here = min(16, P.rows - (rt + r) * 16);
@@ -491,16 +540,28 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
         float l = lsum[r];
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
+        l = over_tiles(l);
         float z[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             z[g] = zacc[r][g] + __shfl_xor(zacc[r][g], 16, 64);
             z[g] += __shfl_xor(z[g], 32, 64);
+            z[g] = over_tiles(z[g]);
+        }
+        if constexpr (C > 1) {
+#pragma unroll
+            for (int j = 0; j < DT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    acc[r][j][e] += __shfl_xor(acc[r][j][e], 32, 64);
+                    if constexpr (C >= 4) acc[r][j][e] += __shfl_xor(acc[r][j][e], 16, 64);
+                }
         }
         float *const po = part_o + r * (2 * 16 * D), *const pml = part_ml + r * (2 * 32);
+        const int part = C == 4 ? qd : C == 2 ? qd >> 1 : 0;  // lanes with the same rows share the dims out
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int row = 4 * qd + e;
+            const int row = (4 * qd + e) % R16;
             const float le = __shfl(l, row, 64), inv = le > 0.f ? 1.f / le : le != le ? le : 0.f;
             float ze[NG];
 #pragma unroll
@@ -509,6 +570,7 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
             const int64_t off = out_row_offset(P, b, kvh, (rt + r) * 16 + row, D) + 2 * pc;
 #pragma unroll
             for (int u = 0; u < D / 32; ++u) {
+                if (C > 1 && u % C != part) continue;
                 const float v0 = acc[r][2 * u][e] + ze[2 * u / GT], v1 = acc[r][2 * u + 1][e] + ze[2 * u / GT];
                 if (whole)
                     int4_store2<EXACT>(P.out, off + 32 * u, le != 0.f ? v0 * inv : 0.f, le != 0.f ? v1 * inv : 0.f, f16);
@@ -516,7 +578,7 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
                     *reinterpret_cast<f32x2_t *>(po + row * D + 32 * u + 2 * pc) = (f32x2_t){v0, v1};
             }
         }
-        if (!whole && qd == 0) {
+        if (!whole && qd == 0 && tq == 0) {
             pml[pc] = fy[r] == -INFINITY ? kNegClamp : -nf[r] * kLn2;
             pml[16 + pc] = l;
         }
@@ -524,7 +586,7 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
 }
 
 // One wave per worker, RTW row tiles each; work lists as in pa_decode_kernel.
-template <int D, int NG, int RTW, bool EXACT>
+template <int D, int NG, int RTW, int C, bool EXACT>
 __global__ void __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2)))
 pa_int4_kernel(const KernelParams P) {
     __shared__ __attribute__((aligned(16))) char lds[int4_wave_lds<NG, EXACT>()];
@@ -549,7 +611,7 @@ pa_int4_kernel(const KernelParams P) {
         const int jt = list_tile0(P, list, b) + j;
         const int kvh = jt / P.row_groups, rg = jt - kvh * P.row_groups;
         const int64_t piece = (int64_t)w * RTW * 2 + slot;
-        run_int4_segment<D, NG, RTW, EXACT>(P, b, kvh, rg * RTW, ctx, blk * bs, min(ctx, (blk + seg) * bs),
+        run_int4_segment<D, NG, RTW, C, EXACT>(P, b, kvh, rg * RTW, ctx, blk * bs, min(ctx, (blk + seg) * bs),
                                             seg == nb, P.part_o + piece * 16 * D, P.part_ml + piece * 32, lds);
         pos += seg;
         slot = 1;
@@ -577,7 +639,7 @@ constexpr int int4_direct_lds() {
     return 16 * D * 4 + 32 * 4 + int4_wave_lds<NG, EXACT>();
 }
 
-template <int D, int NG, typename OutT>
+template <int D, int NG, int C, typename OutT>
 __global__ void __launch_bounds__((64 * int4_direct_waves<D>())) pa_int4_direct_kernel(const KernelParams P) {
     constexpr bool EXACT = std::is_same<OutT, float>::value;
     constexpr int LW = int4_direct_lds<D, NG, EXACT>();
@@ -606,7 +668,7 @@ __global__ void __launch_bounds__((64 * int4_direct_waves<D>())) pa_int4_direct_
     float *const part = reinterpret_cast<float *>(lds);
     const int lo = wave * per, hi = min(chunks, lo + per);
     if (lo < hi)
-        run_int4_segment<D, NG, 1, EXACT>(P, b, kvh, rt, ctx, lo * kInt4Chunk, min(ctx, hi * kInt4Chunk),
+        run_int4_segment<D, NG, 1, C, EXACT>(P, b, kvh, rt, ctx, lo * kInt4Chunk, min(ctx, hi * kInt4Chunk),
                                           chunks <= per, part, part + 16 * D, lds + 16 * D * 4 + 32 * 4);
     const int pieces = (chunks + per - 1) / per;
     if (pieces == 1) return;  // wave 0 stored the output
@@ -614,28 +676,35 @@ __global__ void __launch_bounds__((64 * int4_direct_waves<D>())) pa_int4_direct_
     direct_merge<D, OutT, int4_direct_waves<D>(), LW>(P, b, kvh, rt, units, pieces, int4_lds);
 }
 
-// Two row tiles per wave: not with 256 dims, whose accumulators alone are 128
-// registers then.
+// The kernels for `rows` query rows per kv head. Two row tiles per wave: not
+// with 256 dims, whose accumulators alone are 128 registers then.
 template <int D, int NG, bool EXACT>
-KernelPair int4_set() {
-    if constexpr (D <= 128)
-        return {pa_int4_kernel<D, NG, 1, EXACT>, nullptr, false, false, pa_int4_kernel<D, NG, 2, EXACT>};
-    else
-        return {pa_int4_kernel<D, NG, 1, EXACT>, nullptr, false, false, nullptr};
+KernelPair int4_set(const int rows) {
+    KernelPair k{};
+    k.main = rows <= 4 ? pa_int4_kernel<D, NG, 1, 4, EXACT>
+             : rows <= 8 ? pa_int4_kernel<D, NG, 1, 2, EXACT> : pa_int4_kernel<D, NG, 1, 1, EXACT>;
+    if constexpr (D <= 128) k.main_pair = pa_int4_kernel<D, NG, 2, 1, EXACT>;
+    return k;
 }
 
 template <int D, int NG>
-KernelPair int4_pair(int out_dtype) {
-    return out_dtype == SIMPLER_HIP_DT_FLOAT32 ? int4_set<D, NG, true>() : int4_set<D, NG, false>();
+KernelPair int4_pair(const int rows, const int out_dtype) {
+    return out_dtype == SIMPLER_HIP_DT_FLOAT32 ? int4_set<D, NG, true>(rows) : int4_set<D, NG, false>(rows);
+}
+
+template <int D, int NG, typename OutT>
+DirectFn int4_direct_set(const int rows) {
+    constexpr int lds = int4_direct_lds<D, NG, std::is_same<OutT, float>::value>();
+    return {rows <= 4   ? pa_int4_direct_kernel<D, NG, 4, OutT>
+            : rows <= 8 ? pa_int4_direct_kernel<D, NG, 2, OutT> : pa_int4_direct_kernel<D, NG, 1, OutT>,
+            int4_direct_waves<D>(), lds};
 }
 
 template <int D, int NG>
-DirectFn int4_direct(int out_dtype) {
-    if (out_dtype == SIMPLER_HIP_DT_FLOAT32)
-        return {pa_int4_direct_kernel<D, NG, float>, int4_direct_waves<D>(), int4_direct_lds<D, NG, true>()};
-    if (out_dtype == SIMPLER_HIP_DT_BFLOAT16)
-        return {pa_int4_direct_kernel<D, NG, __bf16>, int4_direct_waves<D>(), int4_direct_lds<D, NG, false>()};
-    return {pa_int4_direct_kernel<D, NG, _Float16>, int4_direct_waves<D>(), int4_direct_lds<D, NG, false>()};
+DirectFn int4_direct(const int rows, const int out_dtype) {
+    return out_dtype == SIMPLER_HIP_DT_FLOAT32    ? int4_direct_set<D, NG, float>(rows)
+           : out_dtype == SIMPLER_HIP_DT_BFLOAT16 ? int4_direct_set<D, NG, __bf16>(rows)
+                                                  : int4_direct_set<D, NG, _Float16>(rows);
 }
 
 }  // namespace pa

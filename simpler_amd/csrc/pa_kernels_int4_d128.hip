@@ -4,20 +4,20 @@
 namespace simpler_hip {
 namespace pa {
 
-KernelPair pick_int4_d128(int groups, int out_dtype) {
+KernelPair pick_int4_d128(int groups, int rows, int out_dtype) {
     switch (groups) {
-        case 1: return int4_pair<128, 1>(out_dtype);
-        case 2: return int4_pair<128, 2>(out_dtype);
-        case 4: return int4_pair<128, 4>(out_dtype);
+        case 1: return int4_pair<128, 1>(rows, out_dtype);
+        case 2: return int4_pair<128, 2>(rows, out_dtype);
+        case 4: return int4_pair<128, 4>(rows, out_dtype);
         default: return KernelPair{};
     }
 }
 
-DirectFn pick_int4_direct_d128(int groups, int out_dtype) {
+DirectFn pick_int4_direct_d128(int groups, int rows, int out_dtype) {
     switch (groups) {
-        case 1: return int4_direct<128, 1>(out_dtype);
-        case 2: return int4_direct<128, 2>(out_dtype);
-        case 4: return int4_direct<128, 4>(out_dtype);
+        case 1: return int4_direct<128, 1>(rows, out_dtype);
+        case 2: return int4_direct<128, 2>(rows, out_dtype);
+        case 4: return int4_direct<128, 4>(rows, out_dtype);
         default: return DirectFn{};
     }
 }

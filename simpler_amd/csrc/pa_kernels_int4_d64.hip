@@ -4,18 +4,18 @@
 namespace simpler_hip {
 namespace pa {
 
-KernelPair pick_int4_d64(int groups, int out_dtype) {
+KernelPair pick_int4_d64(int groups, int rows, int out_dtype) {
     switch (groups) {
-        case 1: return int4_pair<64, 1>(out_dtype);
-        case 2: return int4_pair<64, 2>(out_dtype);
+        case 1: return int4_pair<64, 1>(rows, out_dtype);
+        case 2: return int4_pair<64, 2>(rows, out_dtype);
         default: return KernelPair{};
     }
 }
 
-DirectFn pick_int4_direct_d64(int groups, int out_dtype) {
+DirectFn pick_int4_direct_d64(int groups, int rows, int out_dtype) {
     switch (groups) {
-        case 1: return int4_direct<64, 1>(out_dtype);
-        case 2: return int4_direct<64, 2>(out_dtype);
+        case 1: return int4_direct<64, 1>(rows, out_dtype);
+        case 2: return int4_direct<64, 2>(rows, out_dtype);
         default: return DirectFn{};
     }
 }

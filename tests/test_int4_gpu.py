@@ -65,6 +65,20 @@ def test_lengths(lens, device):
                 assert n or (got[b] == 0).all()
 
 
+@pytest.mark.parametrize("batch", [3, 200, 300, 700])
+@pytest.mark.parametrize("heads", [2, 10, 18])
+def test_short_sequences_by_the_thousand(batch, heads, device):
+    """Tiles few and many: the workgroups of a short batch shrink from eight waves to one."""
+    rng = np.random.default_rng(batch)
+    lens = [int(n) for n in rng.integers(0, 300, batch)]
+    case = make_int4_case(lens, heads=heads, kv_heads=2, dim=64, group=32, block=32, seed=batch + heads)
+    assert pa.kernel_name(pa.make_args(*case.device_args(device)[0], torch.empty_like(case.query, device=device),
+                                       case.scale, k_scale=case.k_scale.to(device),
+                                       v_scale=case.v_scale.to(device))) == "pa_int4_direct_kernel"
+    check(case, device, BF16)
+    check(case, device, FP32)
+
+
 def test_many_sequences_of_mixed_lengths(device):
     rng = np.random.default_rng(3)
     lens = [int(n) for n in rng.integers(0, 90, 600)]
