@@ -3,14 +3,15 @@
 // q/k RMS norm, rotary turn by each pair's own axis, cache write.
 //
 // A byte mover: every projection value is read once and written once in 16
-// bits; the cos/sin rows are shared by a token's heads. A lane holds four pairs
-// (dims 4c .. 4c+3 and those D/2 further), so D/8 lanes hold a head and a wave
-// 4 heads of 128 dims; the turn needs no exchange, the norm's sum one over
-// D/8 lanes. The lane's 16 cos/sin values are loaded once and stay in
-// registers for all the heads that the wave takes of its token: many where
-// there are tokens enough to fill the card, one set of heads where there are
-// few (heads_per_wave). Head dims other than 64, 128 and 256 take a wave per
-// head, elements of a half side by side.
+// bits; the cos/sin rows are shared by a token's heads. A lane holds eight pairs
+// (dims 8c .. 8c+7 and those D/2 further: 16-byte loads and stores), so D/16
+// lanes hold a head and a wave 8 heads of 128 dims; the turn needs no exchange,
+// the norm's sum one over D/16 lanes. A wave works on one token, whose cos/sin
+// rows it gathers by axis into LDS once (a lane per pair) while its first heads'
+// loads are in flight, and goes through the token's heads with kAhead sets of
+// them loaded ahead: all of them where there are tokens enough to fill the
+// card, one set where there are few (sets_per_wave). Head dims other than 64,
+// 128 and 256 take a wave per head, elements of a half side by side.
 //
 // fp32 arithmetic in the golden's order without fused multiply-adds, as in
 // kv_cache.hip (simpler_setup/goldens/qwen3_14b_decode.py:99-103,207-226).
@@ -28,8 +29,6 @@ namespace simpler_hip_kv {
 namespace {
 
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kThreadsR = 256;
 constexpr int kMaxDim = 1024;
@@ -77,20 +76,25 @@ __device__ __forceinline__ float load1(const void *p, const int64_t i) {
     return (float)((const _Float16 *)p)[i];
 }
 
+// Eight values from two 16-byte pieces (fp32) or one.
 template <int T>
-__device__ __forceinline__ f32x4_t load4(const void *p, const int64_t i) {
-    if constexpr (T == kF32) {
-        return *reinterpret_cast<const f32x4_t *>((const float *)p + i);
-    } else {
-        const u32x2_t w = *reinterpret_cast<const u32x2_t *>((const uint16_t *)p + i);
-        if constexpr (T == kBf16)
-            return (f32x4_t){__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u),
-                             __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
-        return (f32x4_t){(float)__builtin_bit_cast(_Float16, (uint16_t)(w[0] & 0xffffu)),
-                         (float)__builtin_bit_cast(_Float16, (uint16_t)(w[0] >> 16)),
-                         (float)__builtin_bit_cast(_Float16, (uint16_t)(w[1] & 0xffffu)),
-                         (float)__builtin_bit_cast(_Float16, (uint16_t)(w[1] >> 16))};
+__device__ __forceinline__ void unpack8(const u32x4_t *w, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (T == kF32) {
+            x[i] = __uint_as_float(w[i / 4][i % 4]);
+        } else {
+            const unsigned b = w[0][i / 2] >> (16 * (i % 2));
+            x[i] = T == kBf16 ? __uint_as_float(b << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)b);
+        }
     }
+}
+
+__device__ __forceinline__ u32x4_t pack8(const float (&x)[8], const bool f16) {
+    u32x4_t w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = round16(x[2 * i], f16) | (unsigned)round16(x[2 * i + 1], f16) << 16;
+    return w;
 }
 
 // A token's place: whether its positions are usable (ok), and its cache rows
@@ -99,20 +103,24 @@ __device__ __forceinline__ f32x4_t load4(const void *p, const int64_t i) {
 struct Place {
     bool ok, write;
     int blk, off;
+    int p0, p1, p2, p3;  // its positions, 0 where not ok
 };
+static_assert(SIMPLER_HIP_MROPE_MAX_AXES == 4, "a token's positions");
 
 __device__ __forceinline__ Place place_of(const RotaryParams &P, const int t, const bool count) {
-    Place r{true, true, 0, t};
-    bool bad = false;
-#pragma unroll
-    for (int a = 0; a < SIMPLER_HIP_MROPE_MAX_AXES; ++a)
-        if (a < P.axes) {
-            const int p = P.pos[(int64_t)a * P.tokens + t];
-            if (a == 0 && p < 0) return Place{false, false, 0, 0};  // padding, whatever the rest says
-            bad |= P.sect[a] > 0 && (p < 0 || p >= P.max_pos);
-        }
-    r.ok = !bad;
-    if (P.slot) {
+    Place r;
+    r.blk = 0;
+    r.off = t;
+    r.p0 = P.pos[t];
+    r.p1 = P.axes > 1 ? P.pos[(int64_t)P.tokens + t] : 0;
+    r.p2 = P.axes > 2 ? P.pos[2 * (int64_t)P.tokens + t] : 0;
+    r.p3 = P.axes > 3 ? P.pos[3 * (int64_t)P.tokens + t] : 0;
+    const bool padding = r.p0 < 0;  // whatever the rest says
+    auto outside = [&](const int a, const int p) { return P.sect[a] > 0 && (unsigned)p >= (unsigned)P.max_pos; };
+    bool bad = !padding && (outside(0, r.p0) || outside(1, r.p1) || outside(2, r.p2) || outside(3, r.p3));
+    r.ok = r.write = !bad && !padding;
+    if (!r.ok) r.p0 = r.p1 = r.p2 = r.p3 = 0;
+    if (P.slot && !padding) {
         const int slot = P.slot[t];
         r.write = slot >= 0;
         if (r.write) {
@@ -129,96 +137,132 @@ __device__ __forceinline__ Place place_of(const RotaryParams &P, const int t, co
     return r;
 }
 
-// D: 64, 128 or 256. A wave: one token, sets_per_wave sets of 512 / D heads
+__device__ __forceinline__ int pos_of(const RotaryParams &P, const Place &at, const int pair) {
+    const int axis = axis_of(P, pair);
+    return axis == 0 ? at.p0 : axis == 1 ? at.p1 : axis == 2 ? at.p2 : at.p3;
+}
+
+// D: 64, 128 or 256. A wave: one token, sets_per_wave sets of 1024 / D heads
 // (q, then k, then v heads).
 template <int D, int T>
 __global__ void __launch_bounds__(kThreadsR) mrope_kernel(const RotaryParams P) {
 #pragma clang fp contract(off)
-    constexpr int L = D / 8, H = 64 / L, half = D / 2;
+    constexpr int L = D / 16, H = 64 / L, half = D / 2;
+    constexpr int kPieces = T == kF32 ? 2 : 1;  // 16-byte loads per eight values
+    constexpr int kAhead = T == kF32 ? 2 : 3;
+    __shared__ __attribute__((aligned(16))) float staged[kThreadsR / 64][4 * D];  // cos, sin, q's and k's weights
     const int lane = threadIdx.x & 63, c = lane % L, sub = lane / L;
+    float *const lds = staged[threadIdx.x >> 6];
     const int waves = (P.sets + P.sets_per_wave - 1) / P.sets_per_wave;  // per token
     const unsigned wave = blockIdx.x * (kThreadsR / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = (int)(wave / (unsigned)waves), part = (int)(wave - (unsigned)t * waves);
     if (t >= P.tokens) return;
-    const Place at = place_of(P, t, part == 0 && lane == 0);
-    const float inv = P.inv_rms ? P.inv_rms[t] : 1.f;
-    // this lane's pairs 4c .. 4c+3: their turns
-    float cl[4], sl[4], ch[4], sh[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int pair = 4 * c + i;
-        const int p = at.ok ? P.pos[(int64_t)axis_of(P, pair) * P.tokens + t] : 0;
-        const float *cr = P.cos + (int64_t)p * D, *sr = P.sin + (int64_t)p * D;
-        cl[i] = cr[pair];
-        sl[i] = sr[pair];
-        ch[i] = cr[pair + half];
-        sh[i] = sr[pair + half];
-    }
-    f32x4_t wq[2], wk[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        wq[s] = P.q_w ? *reinterpret_cast<const f32x4_t *>(P.q_w + 4 * c + s * half) : (f32x4_t){1.f, 1.f, 1.f, 1.f};
-        wk[s] = P.k_w ? *reinterpret_cast<const f32x4_t *>(P.k_w + 4 * c + s * half) : (f32x4_t){1.f, 1.f, 1.f, 1.f};
-    }
     const int heads = P.hq + 2 * P.hkv;
     const int set0 = part * P.sets_per_wave, set1 = min(P.sets, set0 + P.sets_per_wave);
-    auto load = [&](const int set, f32x4_t &lo, f32x4_t &hi) {
+    struct Raw {
+        u32x4_t lo[kPieces], hi[kPieces];
+    };
+    auto load = [&](const int set) {
         const int u = min(set * H + sub, heads - 1);
         const bool is_q = u < P.hq, is_k = u < P.hq + P.hkv;
         const int h = is_q ? u : is_k ? u - P.hq : u - P.hq - P.hkv;
         const void *src = is_q ? P.q : is_k ? P.k : P.v;
-        const int64_t i = t * (is_q ? P.q_s : is_k ? P.k_s : P.v_s) + (int64_t)h * D + 4 * c;
-        lo = load4<T>(src, i);
-        hi = load4<T>(src, i + half);
+        const int64_t i = t * (is_q ? P.q_s : is_k ? P.k_s : P.v_s) + (int64_t)h * D + 8 * c;
+        const char *const at = (const char *)src + i * (T == kF32 ? 4 : 2);
+        Raw r;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            r.lo[k] = *reinterpret_cast<const u32x4_t *>(at + 16 * k);
+            r.hi[k] = *reinterpret_cast<const u32x4_t *>(at + half * (T == kF32 ? 4 : 2) + 16 * k);
+        }
+        return r;
     };
-    f32x4_t lo, hi, lo2, hi2;
-    load(set0, lo, hi);
-    for (int set = set0; set < set1; ++set) {
-        if (set + 1 < set1) load(set + 1, lo2, hi2);
-        const int u = set * H + sub;
-        const bool in = u < heads, is_q = u < P.hq, is_k = !is_q && u < P.hq + P.hkv;
-        const int h = is_q ? u : is_k ? u - P.hq : u - P.hq - P.hkv;
-        if (P.inv_rms) {
-            lo *= inv;
-            hi *= inv;
-        }
-        const bool norm = is_q ? P.q_w != nullptr : is_k && P.k_w != nullptr;
-        if (__any(norm)) {
-            float ss = 0.f;
+    Raw ahead[kAhead];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                ss += lo[i] * lo[i];
-                ss += hi[i] * hi[i];
+    for (int j = 0; j < kAhead; ++j)
+        if (set0 + j < set1) ahead[j] = load(set0 + j);
+
+    const Place at = place_of(P, t, part == 0 && lane == 0);
+    const float inv = P.inv_rms ? P.inv_rms[t] : 1.f;
+#pragma unroll
+    for (int k = 0; k < (half + 63) / 64; ++k) {
+        const int pair = lane + 64 * k;
+        if (pair < half) {
+            const int64_t row = (int64_t)pos_of(P, at, pair) * D + pair;
+            lds[pair] = P.cos[row];
+            lds[pair + half] = P.cos[row + half];
+            lds[D + pair] = P.sin[row];
+            lds[D + pair + half] = P.sin[row + half];
+        }
+    }
+    if (P.q_w || P.k_w) {
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) {
+            const int i = lane + 64 * k;
+            lds[2 * D + i] = P.q_w ? P.q_w[i] : 1.f;
+            lds[3 * D + i] = P.k_w ? P.k_w[i] : 1.f;
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's own LDS writes, in order
+    __builtin_amdgcn_wave_barrier();
+
+    for (int base = set0; base < set1; base += kAhead) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int set = base + j;
+            if (set >= set1) break;
+            float lo[8], hi[8];
+            unpack8<T>(ahead[j].lo, lo);
+            unpack8<T>(ahead[j].hi, hi);
+            if (set + kAhead < set1) ahead[j] = load(set + kAhead);
+            const int u = set * H + sub;
+            const bool in = u < heads, is_q = u < P.hq, is_k = !is_q && u < P.hq + P.hkv;
+            const int h = is_q ? u : is_k ? u - P.hq : u - P.hq - P.hkv;
+            if (P.inv_rms) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    lo[i] *= inv;
+                    hi[i] *= inv;
+                }
             }
+            asm volatile("" ::: "memory");  // the staged values are read per set: kept, they would take half the registers
+            const bool norm = is_q ? P.q_w != nullptr : is_k && P.k_w != nullptr;
+            if (__any(norm)) {
+                float ss = 0.f;
 #pragma unroll
-            for (int d = 1; d < L; d <<= 1) ss += __shfl_xor(ss, d, 64);
-            if (norm) {
-                const float r = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)D) + P.eps));
-                lo = (lo * r) * (is_q ? wq[0] : wk[0]);
-                hi = (hi * r) * (is_q ? wq[1] : wk[1]);
+                for (int i = 0; i < 8; ++i) {
+                    ss += lo[i] * lo[i];
+                    ss += hi[i] * hi[i];
+                }
+#pragma unroll
+                for (int d = 1; d < L; d <<= 1) ss += __shfl_xor(ss, d, 64);
+                if (norm) {
+                    const float r = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)D) + P.eps));
+                    const float *const w = lds + (is_q ? 2 * D : 3 * D) + 8 * c;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        lo[i] = (lo[i] * r) * w[i];
+                        hi[i] = (hi[i] * r) * w[half + i];
+                    }
+                }
+            }
+            if (is_q || is_k) {
+                const float *const cs = lds + 8 * c, *const sn = lds + D + 8 * c;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = lo[i] * cs[i] - hi[i] * sn[i];
+                    hi[i] = hi[i] * cs[half + i] + lo[i] * sn[half + i];
+                    lo[i] = x;
+                }
+            }
+            if (in && (is_q || at.write)) {
+                uint16_t *dst = is_q   ? P.q_out + ((int64_t)t * P.hq + h) * D
+                                : is_k ? P.kc + at.blk * P.k_bs + at.off * P.k_ts + h * P.k_hs
+                                       : P.vc + at.blk * P.v_bs + at.off * P.v_ts + h * P.v_hs;
+                *reinterpret_cast<u32x4_t *>(dst + 8 * c) = at.ok ? pack8(lo, P.f16) : (u32x4_t){0, 0, 0, 0};
+                *reinterpret_cast<u32x4_t *>(dst + 8 * c + half) = at.ok ? pack8(hi, P.f16) : (u32x4_t){0, 0, 0, 0};
             }
         }
-        float o[2][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool turn = is_q || is_k;
-            o[0][i] = turn ? lo[i] * cl[i] - hi[i] * sl[i] : lo[i];
-            o[1][i] = turn ? hi[i] * ch[i] + lo[i] * sh[i] : hi[i];
-            if (!at.ok) o[0][i] = o[1][i] = 0.f;
-        }
-        if (in && (is_q || at.write)) {
-            uint16_t *dst = is_q   ? P.q_out + ((int64_t)t * P.hq + h) * D
-                            : is_k ? P.kc + at.blk * P.k_bs + at.off * P.k_ts + h * P.k_hs
-                                   : P.vc + at.blk * P.v_bs + at.off * P.v_ts + h * P.v_hs;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const u32x2_t w = {round16(o[s][0], P.f16) | (unsigned)round16(o[s][1], P.f16) << 16,
-                                   round16(o[s][2], P.f16) | (unsigned)round16(o[s][3], P.f16) << 16};
-                *reinterpret_cast<u32x2_t *>(dst + 4 * c + s * half) = w;
-            }
-        }
-        lo = lo2;
-        hi = hi2;
     }
 }
 
@@ -273,7 +317,7 @@ __global__ void __launch_bounds__(64) mrope_any_kernel(const RotaryParams P) {
             b = (b * r) * w[i + half];
         }
         if (is_q || is_k) {
-            const int p = at.ok ? P.pos[(int64_t)axis_of(P, i) * P.tokens + t] : 0;
+            const int p = pos_of(P, at, i);
             const float *cr = P.cos + (int64_t)p * P.d, *sr = P.sin + (int64_t)p * P.d;
             const float x = a * cr[i] - b * sr[i];
             b = b * cr[i + half] + a * sr[i + half];
@@ -375,13 +419,11 @@ extern "C" int simpler_hip_qk_norm_mrope_append(const SimplerHipQkNormMropeArgs 
     for (int i = 0; i < a->num_axes; ++i) P.sect[i] = a->sections[i];
     P.f16 = f16;
     P.eps = a->eps;
-    const int esz = a->proj_dtype == SIMPLER_HIP_DT_FLOAT32 ? 4 : 2;
-    // The vector form: four elements per load and store.
+    // The vector form: 16 bytes per load and store.
     bool vec = a->head_dim == 64 || a->head_dim == 128 || a->head_dim == 256;
-    for (int64_t s : strides) vec &= s % 4 == 0;
-    vec &= !unaligned(a->q_proj, 4 * esz) && !unaligned(a->k_proj, 4 * esz) && !unaligned(a->v_proj, 4 * esz);
-    vec &= !unaligned(a->q_out, 8) && !unaligned(a->key_cache, 8) && !unaligned(a->value_cache, 8);
-    vec &= !unaligned(a->q_norm_weight, 16) && !unaligned(a->k_norm_weight, 16);
+    for (int64_t s : strides) vec &= s % 8 == 0;
+    const void *const aligned[6] = {a->q_proj, a->k_proj, a->v_proj, a->q_out, a->key_cache, a->value_cache};
+    for (const void *p : aligned) vec &= !unaligned(p, 16);
     const int64_t heads = (int64_t)a->num_heads + 2 * (int64_t)a->num_kv_heads;
     const RotaryFn fn = a->proj_dtype == SIMPLER_HIP_DT_FLOAT32    ? pick_rotary<kF32>(a->head_dim, vec)
                         : a->proj_dtype == SIMPLER_HIP_DT_BFLOAT16 ? pick_rotary<kBf16>(a->head_dim, vec)
@@ -389,7 +431,7 @@ extern "C" int simpler_hip_qk_norm_mrope_append(const SimplerHipQkNormMropeArgs 
     int64_t groups;
     int threads = 64;
     if (vec) {
-        const int per = 512 / a->head_dim;
+        const int per = 1024 / a->head_dim;
         P.sets = (int)((heads + per - 1) / per);
         P.sets_per_wave = sets_per_wave(a->num_tokens, P.sets);
         const int64_t waves = (int64_t)a->num_tokens * ((P.sets + P.sets_per_wave - 1) / P.sets_per_wave);
