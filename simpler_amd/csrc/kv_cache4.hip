@@ -8,11 +8,14 @@
 // consecutive bytes of a page. K's word goes out as it is; V's four bytes are
 // traded within the row's lanes for two 16-bit pieces each (dims 32 apart).
 //
-// Quantisation. Least and greatest value of a group by DPP moves over its G / 8
-// lanes. The code is round((x - z) / s): (x - z) times a reciprocal of s is
-// within 2^-17 of the quotient, so only where it falls closer than 2^-16 to a
-// half is the quotient compared with that half exactly, in fp64 ((c + 1/2) s has
-// 16 bits); the division itself would cost more than the rest together.
+// Quantisation, whose instructions bound the append. Least and greatest value of
+// a group by DPP moves over its G / 8 lanes. The code is round((x - z) / s):
+// (x - z) times the reciprocal of 15 s, kept in 0 .. 1 (the product's clamp), is
+// within 2^-22 of its value, 15 times it within 2^-18 of the quotient, so only
+// where that falls closer than 2^-16 to a half is the quotient compared with the
+// half exactly, in fp64 ((c + 1/2) s has 16 bits). The code is rounded off by a
+// sum with 1.5 2^23, and eight of those sums make the word, the constants'
+// share taken off at its end.
 
 #include <hip/hip_runtime.h>
 
@@ -27,6 +30,7 @@ namespace {
 
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads4 = 256;
 
@@ -57,10 +61,20 @@ __device__ __forceinline__ T combine_lanes(T x, F f) {
     return x;
 }
 
+__device__ __forceinline__ float min2(const float a, const float b) { return fminf(a, b); }
+__device__ __forceinline__ float max2(const float a, const float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float min3(const float a, const float b, const float c) { return fminf(fminf(a, b), c); }
+__device__ __forceinline__ float max3(const float a, const float b, const float c) { return fmaxf(fmaxf(a, b), c); }
+
 template <bool F16>
 __device__ __forceinline__ float elem_to_float(const unsigned bits16) {
     if constexpr (F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)bits16);
     return __uint_as_float(bits16 << 16);
+}
+
+__device__ __forceinline__ float elem(const u32x4_t &raw, const int i, const bool f16) {
+    const unsigned b = raw[i / 2] >> (16 * (i & 1));
+    return f16 ? elem_to_float<true>(b & 0xffffu) : __uint_as_float(b << 16);
 }
 
 // The lane's eight values, their group's (s, z) pair and the codes' word.
@@ -68,48 +82,54 @@ template <int LANES, bool F16>
 __device__ __forceinline__ void quantise8(const u32x4_t raw, unsigned &word, unsigned &sz) {
 #pragma clang fp contract(off)
     float x[8];
-    unsigned mag = 0;  // largest magnitude's bits: an exponent of ones is not finite
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = elem_to_float<F16>(raw[i] & 0xffffu);
-        x[2 * i + 1] = elem_to_float<F16>(raw[i] >> 16);
-        mag = max(mag, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
-    }
-    float lo = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
-    float hi = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    lo = combine_lanes<LANES>(lo, [](float a, float b) { return fminf(a, b); });
-    hi = combine_lanes<LANES>(hi, [](float a, float b) { return fmaxf(a, b); });
-    mag = combine_lanes<LANES>(mag, [](unsigned a, unsigned b) { return max(a, b); });
-    const bool finite = mag < (F16 ? 0x7c00u : 0x7f80u);
-    const _Float16 zh = (_Float16)fminf(fmaxf(lo, -65504.f), 65504.f);
-    const _Float16 sh = (_Float16)fminf(__fdiv_rn(hi - lo, 15.f), 65504.f);
+    for (int i = 0; i < 8; ++i) x[i] = elem(raw, i, F16);
+    u16x2_t mag = {0, 0};  // largest magnitudes' bits: an exponent of ones is not finite
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        mag = __builtin_elementwise_max(mag, __builtin_bit_cast(u16x2_t, raw[i] & 0x7fff7fffu));
+    const uint64_t odd = __ballot(max(mag[0], mag[1]) >= (F16 ? 0x7c00u : 0x7f80u));
+    float lo = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), min2(x[6], x[7]));
+    float hi = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max2(x[6], x[7]));
+    lo = combine_lanes<LANES>(lo, [](float a, float b) { return min2(a, b); });
+    hi = combine_lanes<LANES>(hi, [](float a, float b) { return max2(a, b); });
+    const _Float16 zh = (_Float16)__builtin_amdgcn_fmed3f(lo, -65504.f, 65504.f);
+    // (hi - lo) / 15, correctly rounded: a quotient within an ulp and its exact remainder
+    constexpr float kFifteenth = 1.f / 15.f;
+    const float range = hi - lo, q0 = range * kFifteenth;
+    const _Float16 sh = (_Float16)fminf(__builtin_fmaf(__builtin_fmaf(-15.f, q0, range), kFifteenth, q0), 65504.f);
     const float z = (float)zh, s = (float)sh;
-    const float inv = s > 0.f ? __builtin_amdgcn_rcpf(s) : 0.f;  // s >= 2^-24: a normal fp32 number
-    word = 0;
-    bool near = false;
-    float r[8];
+    const float inv = s > 0.f ? __builtin_amdgcn_rcpf(15.f * s) : 0.f;  // s >= 2^-24: a normal fp32 number
+    constexpr float kMagic = 12582912.f;  // 1.5 2^23: its sum with a code has the code in its last bits
+    unsigned acc = 0;
+    float off = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        r[i] = fminf(fmaxf((x[i] - z) * inv, 0.f), 15.f);
-        near |= fabsf(r[i] - floorf(r[i]) - 0.5f) < 0x1p-16f;
-        word |= (unsigned)__builtin_rintf(r[i]) << (4 * i);
+    for (int i = 7; i >= 0; --i) {
+        const float r = __builtin_amdgcn_fmed3f((x[i] - z) * inv, 0.f, 1.f);
+        const float t = __builtin_fmaf(r, 15.f, kMagic);
+        off = fmaxf(off, fabsf(__builtin_fmaf(r, 15.f, kMagic - t)));
+        acc = (acc << 4) + __float_as_uint(t);
     }
-    if (near && finite) {
+    word = acc - 0x4b400000u * 0x11111111u;  // kMagic's bits, 8 times
+    sz = (unsigned)__builtin_bit_cast(uint16_t, sh) | (unsigned)__builtin_bit_cast(uint16_t, zh) << 16;
+    if (off > 0.5f - 0x1p-16f) {
         word = 0;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 8; ++i) {
-            const float below = floorf(r[i]);
-            unsigned c = (unsigned)__builtin_rintf(r[i]);
-            if (fabsf(r[i] - below - 0.5f) < 0x1p-16f) {
-                const double d = (double)x[i] - (double)z, half = ((double)below + 0.5) * (double)s;
+            const float v = elem(raw, i, F16), r = __builtin_amdgcn_fmed3f((v - z) * inv, 0.f, 1.f) * 15.f;
+            const float below = floorf(r);
+            unsigned c = (unsigned)__builtin_rintf(r);
+            if (fabsf(r - below - 0.5f) < 0x1p-15f) {
+                const double d = (double)v - (double)z, half = ((double)below + 0.5) * (double)s;
                 c = (unsigned)below + (d > half || (d == half && ((unsigned)below & 1)) ? 1u : 0u);
             }
             word |= c << (4 * i);
         }
     }
-    if (!finite) word = 0;
-    sz = finite ? (unsigned)__builtin_bit_cast(uint16_t, sh) | (unsigned)__builtin_bit_cast(uint16_t, zh) << 16
-                : 0x7e007e00u;
+    if (odd && (odd >> (threadIdx.x & 63 & -LANES) & ((1u << LANES) - 1u))) {
+        word = 0;
+        sz = 0x7e007e00u;
+    }
 }
 
 // Byte offset in a V page of the 16-bit piece of row t that holds dims 64 h + 32 u + 2 l + v.
@@ -118,22 +138,36 @@ __device__ __forceinline__ int v_piece(const int t, const int l, const int h) {
     return ((t >> 2) * 16 + l) * (D / 8) + 4 * (h + (D / 64) * ((t >> 1) & 1)) + 2 * (t & 1);
 }
 
-// grid: x = groups of kRows tokens, y = kv head, z = K or V
+// A thread: dims 8c .. 8c+7 of K and V of a token and kv head. Workgroups of one
+// head after the other over the same kRows tokens, so what runs at once reads
+// whole token rows.
+template <int D>
+struct Share {
+    static constexpr int kLanes = D / 8, kRows = kThreads4 / kLanes;
+    int c, t, h;
+    __device__ explicit Share(const int hkv)
+        : c(threadIdx.x % kLanes), t((int)(blockIdx.x / (unsigned)hkv) * kRows + (int)threadIdx.x / kLanes),
+          h((int)(blockIdx.x % (unsigned)hkv)) {}
+};
+
 template <int D, int G, bool F16>
 __global__ void __launch_bounds__(kThreads4) kv4_append_kernel(const Kv4Params P) {
-    constexpr int L = D / 8, NG = D / G, kRows = kThreads4 / L;
-    const int c = threadIdx.x % L;  // dims 8c .. 8c+7
-    const int t = blockIdx.x * kRows + threadIdx.x / L, h = blockIdx.y;
-    const bool is_k = blockIdx.z == 0;
+    constexpr int NG = D / G;
+    const Share<D> me(P.hkv);
+    const int c = me.c, t = me.t, h = me.h;
     const int bs = 1 << P.bs_shift;
     const bool in = t < P.tokens;
+    const int64_t row = in ? t : 0;
+    const u32x4_t k_raw = *reinterpret_cast<const u32x4_t *>((const uint16_t *)P.key + row * P.key_ts + h * P.key_hs + 8 * c);
+    const u32x4_t v_raw =
+        *reinterpret_cast<const u32x4_t *>((const uint16_t *)P.value + row * P.val_ts + h * P.val_hs + 8 * c);
     int blk = -1, off = 0;
     if (in) {
         if (P.pg.block_table) {
             const int b = t / P.pg.q_len;
             const int64_t p = (int64_t)P.pg.context_lens[b] - P.pg.q_len + (t - b * P.pg.q_len);
             if (p < 0) {
-                if (c == 0 && h == 0 && is_k) atomicOr(P.pg.error_flag, P.pg.bad_length);
+                if (c == 0 && h == 0) atomicOr(P.pg.error_flag, P.pg.bad_length);
             } else if (p < (int64_t)P.pg.max_blocks << P.bs_shift) {
                 const int phys = P.pg.block_table[(int64_t)b * P.pg.max_blocks + (p >> P.bs_shift)];
                 if ((unsigned)phys < (unsigned)P.num_blocks) blk = phys;  // else reported when the decode reads it
@@ -145,71 +179,43 @@ __global__ void __launch_bounds__(kThreads4) kv4_append_kernel(const Kv4Params P
                 blk = slot >> P.bs_shift;
                 off = slot & (bs - 1);
                 if (blk >= P.num_blocks) {
-                    if (c == 0 && h == 0 && is_k && P.err) atomicAdd(P.err, 1);
+                    if (c == 0 && h == 0 && P.err) atomicAdd(P.err, 1);
                     blk = -1;
                 }
             }
         }
     }
-    const uint16_t *src = is_k ? (const uint16_t *)P.key + (in ? t : 0) * P.key_ts + h * P.key_hs
-                               : (const uint16_t *)P.value + (in ? t : 0) * P.val_ts + h * P.val_hs;
-    unsigned word, sz;
-    quantise8<G / 8, F16>(*reinterpret_cast<const u32x4_t *>(src + 8 * c), word, sz);
+    unsigned k_word, k_sz, v_word, v_sz;
+    quantise8<G / 8, F16>(k_raw, k_word, k_sz);
+    quantise8<G / 8, F16>(v_raw, v_word, v_sz);
     // V: lane c's byte i is the nibbles 2u, 2u+1 of piece (4 (c % 4) + i, c / 8),
     // u = (c / 4) % 2; with the lane 4 away it makes the pieces of two l each
-    const unsigned other = __shfl_xor(word, 4, 64);
+    const unsigned other = __shfl_xor(v_word, 4, 64);
     if (blk < 0) return;
     const int64_t at = (((int64_t)blk * P.hkv + h) * NG + 8 * c / G) * bs + off;
-    if (c % (G / 8) == 0) (is_k ? P.ks : P.vs)[at] = sz;
-    if (is_k) {
-        uint8_t *page = P.kc + blk * P.k_bs + h * P.k_hs;
-        *reinterpret_cast<unsigned *>(page + off * (D / 2) + 4 * ((D / 32) * (c & 3) + (c >> 2))) = word;
-    } else {
-        uint8_t *page = P.vc + blk * P.v_bs + h * P.v_hs;
-        const bool high = c & 4;
-        const unsigned u0 = high ? other : word, u1 = high ? word : other;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int i = 2 * (high ? 1 : 0) + k;
-            const unsigned piece = ((u0 >> (8 * i)) & 0xffu) | ((u1 >> (8 * i)) & 0xffu) << 8;
-            *reinterpret_cast<uint16_t *>(page + v_piece<D>(off, 4 * (c & 3) + i, c >> 3)) = (uint16_t)piece;
-        }
+    if (c % (G / 8) == 0) {
+        P.ks[at] = k_sz;
+        P.vs[at] = v_sz;
     }
+    uint8_t *const kp = P.kc + blk * P.k_bs + h * P.k_hs, *const vp = P.vc + blk * P.v_bs + h * P.v_hs;
+    *reinterpret_cast<unsigned *>(kp + off * (D / 2) + 4 * ((D / 32) * (c & 3) + (c >> 2))) = k_word;
+    const bool high = c & 4;
+    const unsigned u0 = high ? other : v_word, u1 = high ? v_word : other;
+    // bytes 2k and 2k + 1 of u0 and u1, k = high: piece i of u0's byte, then u1's
+    const unsigned both = __builtin_amdgcn_perm(u1, u0, high ? 0x07030602u : 0x05010400u);
+    uint8_t *const piece = vp + v_piece<D>(off, 4 * (c & 3) + (high ? 2 : 0), c >> 3);
+    *reinterpret_cast<uint16_t *>(piece) = (uint16_t)both;
+    *reinterpret_cast<uint16_t *>(piece + D / 8) = (uint16_t)(both >> 16);  // the next l
 }
 
 enum { kRowF32 = 0, kRowBf16 = 1, kRowF16 = 2 };
 
-template <int D, int G, int ROW>
-__global__ void __launch_bounds__(kThreads4) kv4_gather_kernel(const Kv4Params P) {
-    constexpr int L = D / 8, NG = D / G, kRows = kThreads4 / L;
-    const int c = threadIdx.x % L;
-    const int t = blockIdx.x * kRows + threadIdx.x / L, h = blockIdx.y;
-    const bool is_k = blockIdx.z == 0;
-    if (t >= P.tokens) return;
-    const int bs = 1 << P.bs_shift;
-    const int slot = P.slot[t];
-    const int blk = slot >> P.bs_shift, off = slot & (bs - 1);
-    const bool there = slot >= 0 && blk < P.num_blocks;
-    if (slot >= 0 && !there && c == 0 && h == 0 && is_k && P.err) atomicAdd(P.err, 1);
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (there) {
-        const unsigned sz = (is_k ? P.ks : P.vs)[(((int64_t)blk * P.hkv + h) * NG + 8 * c / G) * bs + off];
-        unsigned word;
-        if (is_k) {
-            const uint8_t *page = P.kc + blk * P.k_bs + h * P.k_hs;
-            word = *reinterpret_cast<const unsigned *>(page + off * (D / 2) + 4 * ((D / 32) * (c & 3) + (c >> 2)));
-        } else {
-            const uint8_t *page = P.vc + blk * P.v_bs + h * P.v_hs + ((c >> 2) & 1);
-            word = 0;
+template <int ROW>
+__device__ __forceinline__ void store_row8(void *dst, const int64_t at, const unsigned word, const unsigned sz) {
+    const float s = elem_to_float<true>(sz & 0xffffu), z = elem_to_float<true>(sz >> 16);
+    float x[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) word |= (unsigned)page[v_piece<D>(off, 4 * (c & 3) + i, c >> 3)] << (8 * i);
-        }
-        const float s = elem_to_float<true>(sz & 0xffffu), z = elem_to_float<true>(sz >> 16);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf((float)((word >> (4 * i)) & 15u), s, z);
-    }
-    const int64_t at = (is_k ? t * P.key_ts + h * P.key_hs : t * P.val_ts + h * P.val_hs) + 8 * c;
-    void *dst = is_k ? P.key : P.value;
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf((float)((word >> (4 * i)) & 15u), s, z);
     if constexpr (ROW == kRowF32) {
         *reinterpret_cast<f32x4_t *>((float *)dst + at) = (f32x4_t){x[0], x[1], x[2], x[3]};
         *reinterpret_cast<f32x4_t *>((float *)dst + at + 4) = (f32x4_t){x[4], x[5], x[6], x[7]};
@@ -226,6 +232,35 @@ __global__ void __launch_bounds__(kThreads4) kv4_gather_kernel(const Kv4Params P
         }
         *reinterpret_cast<u32x4_t *>((uint16_t *)dst + at) = w;
     }
+}
+
+template <int D, int G, int ROW>
+__global__ void __launch_bounds__(kThreads4) kv4_gather_kernel(const Kv4Params P) {
+    constexpr int NG = D / G;
+    const Share<D> me(P.hkv);
+    const int c = me.c, t = me.t, h = me.h;
+    const int bs = 1 << P.bs_shift;
+    const int slot = t < P.tokens ? P.slot[t] : -1;
+    const int blk = slot >> P.bs_shift, off = slot & (bs - 1);
+    const bool there = slot >= 0 && blk < P.num_blocks;
+    if (slot >= 0 && !there && c == 0 && h == 0 && P.err) atomicAdd(P.err, 1);
+    unsigned k_word = 0, k_sz = 0, both = 0, v_sz = 0;
+    const bool high = c & 4;
+    if (there) {
+        const int64_t at = (((int64_t)blk * P.hkv + h) * NG + 8 * c / G) * bs + off;
+        k_sz = P.ks[at];
+        v_sz = P.vs[at];
+        const uint8_t *const kp = P.kc + blk * P.k_bs + h * P.k_hs, *const vp = P.vc + blk * P.v_bs + h * P.v_hs;
+        k_word = *reinterpret_cast<const unsigned *>(kp + off * (D / 2) + 4 * ((D / 32) * (c & 3) + (c >> 2)));
+        const uint8_t *const piece = vp + v_piece<D>(off, 4 * (c & 3) + (high ? 2 : 0), c >> 3);
+        both = *reinterpret_cast<const uint16_t *>(piece) | (unsigned)*reinterpret_cast<const uint16_t *>(piece + D / 8) << 16;
+    }
+    // V: the append's trade, back: two pieces hold two bytes of this lane's word and two of the lane 4 away
+    const unsigned other = __shfl_xor(both, 4, 64);
+    if (t >= P.tokens) return;
+    const unsigned v_word = high ? __builtin_amdgcn_perm(both, other, 0x07050301u) : __builtin_amdgcn_perm(other, both, 0x06040200u);
+    store_row8<ROW>(P.key, t * P.key_ts + h * P.key_hs + 8 * c, k_word, k_sz);
+    store_row8<ROW>(P.value, t * P.val_ts + h * P.val_hs + 8 * c, v_word, v_sz);
 }
 
 typedef void (*Kv4Fn)(Kv4Params);
@@ -258,8 +293,9 @@ int block_shift(const int bs) { return bs == 16 ? 4 : bs == 32 ? 5 : bs == 64 ? 
 
 int launch(Kv4Fn fn, const Kv4Params &P, const int d, hipStream_t stream) {
     const int rows = kThreads4 / (d / 8);
-    hipLaunchKernelGGL(fn, dim3((unsigned)((P.tokens + rows - 1) / rows), (unsigned)P.hkv, 2), dim3(kThreads4), 0,
-                       stream, P);
+    const int64_t groups = ((int64_t)P.tokens + rows - 1) / rows * P.hkv;
+    if (groups * kThreads4 >= (int64_t)1 << 32) return SIMPLER_HIP_ERR_UNSUPPORTED;  // a launch's threads
+    hipLaunchKernelGGL(fn, dim3((unsigned)groups), dim3(kThreads4), 0, stream, P);
     return hipGetLastError() == hipSuccess ? SIMPLER_HIP_OK : SIMPLER_HIP_ERR_LAUNCH;
 }
 
