@@ -259,8 +259,10 @@ __global__ void __launch_bounds__(kThreadsR) mrope_kernel(const RotaryParams P) 
                 uint16_t *dst = is_q   ? P.q_out + ((int64_t)t * P.hq + h) * D
                                 : is_k ? P.kc + at.blk * P.k_bs + at.off * P.k_ts + h * P.k_hs
                                        : P.vc + at.blk * P.v_bs + at.off * P.v_ts + h * P.v_hs;
-                *reinterpret_cast<u32x4_t *>(dst + 8 * c) = at.ok ? pack8(lo, P.f16) : (u32x4_t){0, 0, 0, 0};
-                *reinterpret_cast<u32x4_t *>(dst + 8 * c + half) = at.ok ? pack8(hi, P.f16) : (u32x4_t){0, 0, 0, 0};
+                const u32x4_t none = {0, 0, 0, 0};
+                __builtin_nontemporal_store(at.ok ? pack8(lo, P.f16) : none, reinterpret_cast<u32x4_t *>(dst + 8 * c));
+                __builtin_nontemporal_store(at.ok ? pack8(hi, P.f16) : none,
+                                            reinterpret_cast<u32x4_t *>(dst + 8 * c + half));
             }
         }
     }
