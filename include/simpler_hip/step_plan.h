@@ -73,11 +73,12 @@ typedef struct SimplerHipAssignSlotsArgs {
  * it lacks from the top of the stack, free_blocks[free_count - 1] first, request
  * by request. A request gets all of its tokens or none: it is refused where
  * context_lens or new_lens is negative, where its tokens do not fit the table
- * row or end past num_tokens, or where it needs blocks and the stack does not
- * cover it together with every earlier request that passed the other checks.
- * A refused request's tokens keep their place with slot, position and request
- * -1, as do places past the last token; a negative block id gives slot -1; starts hold 2^31 - 1 at most. batch at
- * most SIMPLER_HIP_STEP_MAX_BATCH. */
+ * row (or a length of 2^31 - 1) or end past num_tokens, or where it needs blocks
+ * and the stack does not cover it together with every earlier request that
+ * passed the other checks. A refused request's tokens keep their place with
+ * slot, position and request -1, as do places past the last token; a negative
+ * block id gives slot -1; starts and slots are 2^31 - 1 at most. batch at most
+ * SIMPLER_HIP_STEP_MAX_BATCH. */
 int simpler_hip_assign_slots(const SimplerHipAssignSlotsArgs *args, void *stream);
 
 #pragma GCC visibility pop

@@ -117,7 +117,7 @@ def assign_slots(new, lens, table, free, count, block, num_tokens):
     for b in range(len(lens)):
         n, have = int(new[b]), int(lens[b])
         end = at + max(n, 0)
-        ok = n >= 0 and have >= 0 and have + n <= width * block and end <= num_tokens
+        ok = n >= 0 and have >= 0 and have + n <= min(width * block, 2**31 - 1) and end <= num_tokens
         had = -(-have // block)
         need = -(-(have + n) // block) - had if ok else 0
         if ok and need:
@@ -129,8 +129,9 @@ def assign_slots(new, lens, table, free, count, block, num_tokens):
             left -= need
             for i in range(n):
                 p = have + i
-                phys = table[b, p // block]
-                slots[at + i], pos[at + i], req[at + i] = phys * block + p % block if phys >= 0 else -1, p, b
+                phys = int(table[b, p // block])
+                slots[at + i] = min(phys * block + p % block, 2**31 - 1) if phys >= 0 else -1
+                pos[at + i], req[at + i] = p, b
         granted.append(n if ok else 0)
         out_lens.append(have + n if ok else have)
         at = end

@@ -25,34 +25,53 @@ constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kTokensPerThread = 4;  // consecutive ones: one search for them
 
-__device__ __forceinline__ int64_t wave_scan(int64_t x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
-    }
+// a + b, at most 2^32 - 1: sums that pass it (lengths that no step has) stay there.
+__device__ __forceinline__ unsigned sat_add(const unsigned a, const unsigned b) {
+    return __builtin_elementwise_add_sat(a, b);
+}
+
+// Inclusive sum over the lanes, by DPP moves: within rows of 16, then each row's
+// last lane into the rows after it.
+__device__ __forceinline__ unsigned wave_scan(unsigned x) {
+#define SIMPLER_DPP(ctrl, rows) (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false)
+    x = sat_add(x, SIMPLER_DPP(0x111, 0xf));  // row_shr 1
+    x = sat_add(x, SIMPLER_DPP(0x112, 0xf));  // row_shr 2
+    x = sat_add(x, SIMPLER_DPP(0x114, 0xf));  // row_shr 4
+    x = sat_add(x, SIMPLER_DPP(0x118, 0xf));  // row_shr 8
+    x = sat_add(x, SIMPLER_DPP(0x142, 0xa));  // lane 15 of rows 0 and 2 into rows 1 and 3
+    x = sat_add(x, SIMPLER_DPP(0x143, 0xc));  // lane 31 into rows 2 and 3
+#undef SIMPLER_DPP
     return x;
 }
 
 // Inclusive sum of x over the workgroup's threads; *total: of all of them.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t (&sums)[kWaves], int64_t *total) {
+__device__ __forceinline__ unsigned block_scan(unsigned x, unsigned (&sums)[kWaves], unsigned *total) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     x = wave_scan(x);
     __syncthreads();  // the last use of `sums` is over
     if (lane == 63) sums[wave] = x;
     __syncthreads();
-    int64_t before = 0, all = 0;
+    unsigned before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) before += sums[w];
-        all += sums[w];
+        if (w < wave) before = sat_add(before, sums[w]);
+        all = sat_add(all, sums[w]);
     }
     *total = all;
-    return x + before;
+    return sat_add(before, x);
 }
 
-__device__ __forceinline__ int saturate(const int64_t x) { return (int)min(x, (int64_t)0x7fffffff); }
+__device__ __forceinline__ int saturate(const unsigned x) { return (int)min(x, 0x7fffffffu); }
+
+// Blocks of a length of 0 or more.
+__device__ __forceinline__ int blocks_of(const int len, const int bs) {
+    return (int)(((unsigned)len + (unsigned)(bs - 1)) / (unsigned)bs);
+}
+
+// Tokens that a table row holds, as far as a length counts.
+__device__ __forceinline__ int row_capacity(const int width, const int bs) {
+    return (int)min((int64_t)width * bs, (int64_t)0x7fffffff);
+}
 
 // First index in 0 .. n whose (non-decreasing) value is above x.
 __device__ __forceinline__ int first_above(const int *v, const int n, const int x) {
@@ -75,23 +94,23 @@ struct ReleaseParams {
 
 __global__ void __launch_bounds__(kThreads) release_kernel(const ReleaseParams P) {
     extern __shared__ int upto[];  // blocks given back by requests 0 .. b
-    __shared__ int64_t sums[kWaves];
-    const int64_t cap = (int64_t)P.width * P.bs;
+    __shared__ unsigned sums[kWaves];
+    const int cap = row_capacity(P.width, P.bs);
     const int count = min(max(P.count[0], 0), P.capacity);
-    int64_t carry = 0;
+    unsigned carry = 0;
     int bad = 0;
     for (int base = 0; base < P.batch; base += kThreads) {
         const int b = base + threadIdx.x;
         int n = 0;
-        if (b < P.batch && P.ended[b]) {
-            const int len = P.lens[b];
-            bad += len < 0 || len > cap;
-            n = (int)((min(max((int64_t)len, (int64_t)0), cap) + P.bs - 1) / P.bs);
+        if (b < P.batch) {
+            const int ended = P.ended[b], len = P.lens[b];
+            bad += ended && (len < 0 || len > cap);
+            n = ended ? blocks_of(min(max(len, 0), cap), P.bs) : 0;
         }
-        int64_t total;
-        const int64_t incl = block_scan(n, sums, &total);
-        if (b < P.batch) upto[b] = saturate(carry + incl);
-        carry += total;
+        unsigned total;
+        const unsigned incl = block_scan(n, sums, &total);
+        if (b < P.batch) upto[b] = saturate(sat_add(carry, incl));
+        carry = sat_add(carry, total);
     }
     __syncthreads();
     const int room = P.capacity - count, all = saturate(carry), given = min(all, room);
@@ -118,12 +137,13 @@ struct AssignParams {
 
 __global__ void __launch_bounds__(kThreads) assign_kernel(const AssignParams P) {
     extern __shared__ int lds[];
-    int *const ends = lds;            // tokens of requests 0 .. b
-    int *const upto = lds + P.batch;  // blocks that requests 0 .. b ask for
-    __shared__ int64_t sums[kWaves];
-    const int64_t cap = (int64_t)P.width * P.bs;
+    int *const ends = lds;                // tokens of requests 0 .. b
+    int *const upto = lds + P.batch;      // blocks that requests 0 .. b ask for
+    int *const lens = lds + 2 * P.batch;  // of the requests that get their tokens, else -1
+    __shared__ unsigned sums[kWaves];
+    const int cap = row_capacity(P.width, P.bs);
     const int count = min(max(P.count[0], 0), P.capacity);
-    int64_t tok_carry = 0, blk_carry = 0;
+    unsigned tok_carry = 0, blk_carry = 0;
     int taken = 0;  // by this thread's requests
     int refused = 0;
     const bool lead = blockIdx.x == 0;
@@ -134,18 +154,18 @@ __global__ void __launch_bounds__(kThreads) assign_kernel(const AssignParams P) 
             len = P.lens[b];
             n = P.new_lens[b];
         }
-        int64_t total;
-        const int64_t end = tok_carry + block_scan(max(n, 0), sums, &total);
-        tok_carry += total;
-        const bool fits = n >= 0 && len >= 0 && (int64_t)len + n <= cap && end <= P.tokens;
-        const int had = fits ? (int)(((int64_t)len + P.bs - 1) / P.bs) : 0;
-        const int need = fits ? (int)(((int64_t)len + n + P.bs - 1) / P.bs) - had : 0;
-        const int64_t asked = blk_carry + block_scan(need, sums, &total);
-        blk_carry += total;
+        unsigned total;
+        const unsigned end = sat_add(tok_carry, block_scan(max(n, 0), sums, &total));
+        tok_carry = sat_add(tok_carry, total);
+        const bool fits = n >= 0 && len >= 0 && n <= cap && len <= cap - n && end <= (unsigned)P.tokens;
+        const int need = fits ? blocks_of(len + n, P.bs) - blocks_of(len, P.bs) : 0;
+        const unsigned asked = sat_add(blk_carry, block_scan(need, sums, &total));
+        blk_carry = sat_add(blk_carry, total);
         if (b < P.batch) {
-            const bool ok = fits && (need == 0 || asked <= count);
+            const bool ok = fits && (need == 0 || asked <= (unsigned)count);
             ends[b] = saturate(end);
             upto[b] = saturate(asked);
+            lens[b] = ok ? len : -1;
             if (ok) taken += need;
             refused += !ok;
             if (lead) {
@@ -156,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) assign_kernel(const AssignParams P) 
         }
     }
     if (lead) {
-        int64_t all_taken, all_refused;
+        unsigned all_taken, all_refused;
         (void)block_scan(taken, sums, &all_taken);
         (void)block_scan(refused, sums, &all_refused);
         if (threadIdx.x == 0) {
@@ -167,25 +187,22 @@ __global__ void __launch_bounds__(kThreads) assign_kernel(const AssignParams P) 
     }
     __syncthreads();
 
-    // What request b has, may take and gets, as above.
     struct Request {
         int len, had, first;  // first: blocks asked for before it
         bool ok;
     };
     auto request = [&](const int b) {
-        const int n = P.new_lens[b];
         Request r;
-        r.len = P.lens[b];
+        r.len = lens[b];
+        r.ok = r.len >= 0;
         r.first = b ? upto[b - 1] : 0;
-        r.ok = n >= 0 && r.len >= 0 && (int64_t)r.len + n <= cap && ends[b] <= P.tokens &&
-               (upto[b] == r.first || upto[b] <= count);
-        r.had = (int)(((int64_t)max(r.len, 0) + P.bs - 1) / P.bs);
+        r.had = blocks_of(max(r.len, 0), P.bs);
         return r;
     };
     const int thread = blockIdx.x * kThreads + threadIdx.x, threads = gridDim.x * kThreads;
 
     // the blocks: entry i of all that are asked for, as far as the stack goes
-    const int given = (int)min(blk_carry, (int64_t)count);
+    const int given = (int)min(blk_carry, (unsigned)count);
     for (int i = thread; i < given; i += threads) {
         const int b = first_above(upto, P.batch, i);
         const Request r = request(b);
@@ -215,10 +232,10 @@ __global__ void __launch_bounds__(kThreads) assign_kernel(const AssignParams P) 
             if (t < used && r.ok) {
                 pos = r.len + (t - start);
                 req = b;
-                const int blk = pos / P.bs;
+                const int blk = (int)((unsigned)pos / (unsigned)P.bs);
                 const int phys = blk < r.had ? P.table[(int64_t)b * P.width + blk]
                                              : P.free_blocks[count - 1 - (r.first + blk - r.had)];
-                slot = phys < 0 ? -1 : phys * P.bs + (pos - blk * P.bs);
+                slot = phys < 0 ? -1 : (int)min((int64_t)phys * P.bs + (pos - blk * P.bs), (int64_t)0x7fffffff);
             }
             P.slots[t] = slot;
             P.positions[t] = pos;
@@ -274,7 +291,7 @@ extern "C" int simpler_hip_assign_slots(const SimplerHipAssignSlotsArgs *a, void
                    a->block_size, a->capacity,    a->num_tokens};
     const unsigned grid = grid_for(std::max<int64_t>(((int64_t)a->num_tokens + kTokensPerThread - 1) / kTokensPerThread,
                                                      a->batch));
-    hipLaunchKernelGGL(assign_kernel, dim3(grid), dim3(kThreads), (size_t)std::max(a->batch, 1) * 8,
+    hipLaunchKernelGGL(assign_kernel, dim3(grid), dim3(kThreads), (size_t)std::max(a->batch, 1) * 12,
                        (hipStream_t)stream, P);
     return hipGetLastError() == hipSuccess ? SIMPLER_HIP_OK : SIMPLER_HIP_ERR_LAUNCH;
 }

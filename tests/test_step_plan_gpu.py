@@ -86,6 +86,22 @@ def test_requests_that_are_refused(device):
     assert want[5].tolist() == [2, 0, 2, 0]
 
 
+def test_lengths_and_slots_at_the_end_of_32_bits(device):
+    """A table row that holds more tokens than a length counts; a block id whose slot passes 2^31 - 1."""
+    s = State([3, 3], 4096, 2**19 + 8, 16, seed=5)
+    s.lens[0] = 2**31 - 11
+    s.table[0, -16:] = 0
+    want = check_assign(s, [10, 2], 30, device, refused=0)
+    assert want[4][0] == 2**31 - 1
+    assert check_assign(s, [11, 2], 30, device, refused=1)[5].tolist() == [0, 2]
+    s = State([1, 1], 16, 4, 8, seed=6)
+    s.table[0, 0] = 2**27
+    assert check_assign(s, [3, 3], 6, device, refused=0)[0][0] == 2**31 - 1
+    # prompts whose sum passes 32 bits: those after it have no place
+    s = State([0] * 6, 16, 4, 8, seed=7)
+    check_assign(s, [2**31 - 1, 5, 2**31 - 1, 2**31 - 1, 3, 0], 40, device)
+
+
 def test_free_count_outside_the_list(device):
     s = State([3, 3], 4, 5, 8, seed=3)
     for count, clamped in ((-5, 0), (1000, 8)):
