@@ -30,7 +30,16 @@ using namespace pa;
 constexpr int kZeroOffset = 128;  // workspace bytes [128, 256) are never written after init
 constexpr int kMaxAppendTokens = 16;  // fused append: new tokens per sequence (one per residue mod 16)
 constexpr size_t kMaxZeroPageBytes = 1 << 20;  // larger token strides read the padding tiles as they are
-constexpr int kInt4WavesPerCu = 8;  // 4-bit caches: worker waves per CU
+// 4-bit caches: worker waves per CU, as many as their registers let run (32
+// sequences of 1024 to 8192 tokens 45.0 us, 58 with four).
+constexpr int kInt4WavesPerCu = 8;
+// 4-bit caches: work charged for each tile that a slice starts (its queries, a
+// first chunk without prefetch, its partial), in tokens. Without it the workers
+// that hold the end of one tile and the start of another end last: 32 sequences
+// of 1024 to 8192 tokens 42.7 us against 45.4, 13 of up to 9000 and 32 rows 50.1 / 54.5,
+// 37 of up to 5000 and 64 dims 23.2 / 25.3, 24 of up to 20000 55.3 / 57.3; lengths
+// that share out evenly lose by it, 8 sequences of 32768 57.8 / 56.2.
+constexpr int kInt4SegTokens = 192;
 constexpr int kMlaSegTokens = 256;  // MLA: work charged for each sequence a slice starts, in tokens
 
 struct Plan {
@@ -124,6 +133,9 @@ struct Kernels {
     DirectFn direct;
     MergeFn merge;
 };
+
+// Tokens per unit of the work lists: a chunk of the kernel, or a page.
+int int4_unit(const SimplerHipPaDecodeArgs *a) { return std::min(a->block_size, 64); }
 
 KernelPair pick_int4(int d, int groups, int rows, int out) {
     return d == 64    ? pick_int4_d64(groups, rows, out)
@@ -349,6 +361,7 @@ Plan make_plan(const SimplerHipPaDecodeArgs *a, const KernelPair &k) {  // k: th
             }
         }
         p.grid = p.workers;
+        if (int4) p.seg_cost = kInt4SegTokens / int4_unit(a);
     }
     const int dv = a->head_dim_v;
     // Layout: [error word] [zero page] [m,l partials] [O partials]; two
@@ -654,6 +667,11 @@ int pa_decode_launch(const SimplerHipPaDecodeArgs *a, void *workspace, size_t wo
     P.row_groups = plan.row_groups;
     P.block_size = a->block_size;
     P.max_blocks = a->max_blocks_per_seq;
+    if (is_int4(a)) {
+        P.block_size = int4_unit(a);
+        P.max_blocks = a->max_blocks_per_seq * (a->block_size / P.block_size);
+        P.page_shift = __builtin_ctz((unsigned)a->block_size);
+    }
     P.num_pool_blocks = a->num_blocks;
     P.workers = plan.workers;
     P.lanes = plan.lanes;

@@ -114,7 +114,8 @@ struct KernelParams {
     int32_t batch, q_len, num_heads, kv_heads, group, rows, row_tiles;
     int32_t tiles_per_worker;  // row tiles a worker workgroup runs side by side (one wave each)
     int32_t row_groups;        // ceil(row_tiles / tiles_per_worker): work-list tiles per kv head
-    int32_t block_size, max_blocks, num_pool_blocks;
+    int32_t block_size, max_blocks, num_pool_blocks;  // 4-bit caches: of units of the work lists, 64 tokens or a page
+    int32_t page_shift;  // 4-bit caches: log2 of a page's tokens
     int32_t workers;
     int32_t lanes;  // independent work lists; list u holds tiles [u, u+1) * (tiles per batch / lanes) of each batch
     float scale;

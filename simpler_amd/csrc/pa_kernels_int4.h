@@ -120,7 +120,7 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
     static_assert(C == 1 || RTW == 1, "several row tiles: 16 rows each");
     const int lane = threadIdx.x & 63, qd = lane >> 4, pc = lane & 15;
     const int tq = pc / R16, pr = pc % R16;  // this lane's token tile of a set, its row
-    const int bs = P.block_size, sh = __builtin_ctz(bs);
+    const int sh = P.page_shift, bs = 1 << sh;
     const bool f16 = P.half16;
     // constants of the conversions, kept in registers
     unsigned low = 0x000f000fu, high = 0x00f000f0u, k1024 = 0x64006400u;
@@ -145,7 +145,7 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
         }
     }
     const __attribute__((address_space(4))) int32_t *bt_row =
-        (const __attribute__((address_space(4))) int32_t *)(P.block_table + (int64_t)b * P.max_blocks);
+        (const __attribute__((address_space(4))) int32_t *)(P.block_table + (int64_t)b * (P.max_blocks * P.block_size >> sh));
     const char *k_head = reinterpret_cast<const char *>(P.k) + (int64_t)kvh * P.k_head_stride;
     const char *v_head = reinterpret_cast<const char *>(P.v) + (int64_t)kvh * P.v_head_stride;
     const unsigned *k_sc = reinterpret_cast<const unsigned *>(P.k_scale);
@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2)))
 pa_int4_kernel(const KernelParams P) {
     __shared__ __attribute__((aligned(16))) char lds[int4_wave_lds<NG, EXACT>()];
     flag_bad_lengths(P);
-    const int w = blockIdx.x, bs = P.block_size;
+    const int w = blockIdx.x, unit = P.block_size;
     const int tpb = lane_tiles(P);
     const int list = w % P.lanes;
     int start = 0, end = 0, b = 0, prefix = 0, ctx0 = 0;
@@ -602,27 +602,30 @@ pa_int4_kernel(const KernelParams P) {
     prefix = __builtin_amdgcn_readfirstlane(prefix);
     if (start >= end) return;
     int ctx = __builtin_amdgcn_readfirstlane(ctx0);
-    int nb = (ctx + bs - 1) / bs;
+    int nb = (ctx + unit - 1) / unit;
     if (nb == 0) return;
-    const int rel = start - prefix;
-    int j = rel / nb, blk = rel - j * nb, pos = start, slot = 0;
-    while (pos < end && nb > 0) {
-        const int seg = min(end - pos, nb - blk);
-        const int jt = list_tile0(P, list, b) + j;
-        const int kvh = jt / P.row_groups, rg = jt - kvh * P.row_groups;
-        const int64_t piece = (int64_t)w * RTW * 2 + slot;
-        run_int4_segment<D, NG, RTW, C, EXACT>(P, b, kvh, rg * RTW, ctx, blk * bs, min(ctx, (blk + seg) * bs),
-                                            seg == nb, P.part_o + piece * 16 * D, P.part_ml + piece * 32, lds);
-        pos += seg;
-        slot = 1;
-        if (pos >= end) break;
-        blk = 0;
+    // A tile takes seg_cost units of work, for the set-up and the end of a wave's
+    // part of it, then one per 64 tokens (or smaller page); the slice runs those it holds.
+    int j = (start - prefix) / (nb + P.seg_cost), t0 = prefix + j * (nb + P.seg_cost), slot = 0;
+    while (nb > 0) {
+        const int blk0 = max(0, start - t0 - P.seg_cost), blk1 = min(nb, end - t0 - P.seg_cost);
+        if (blk1 > blk0) {
+            const int jt = list_tile0(P, list, b) + j;
+            const int kvh = jt / P.row_groups, rg = jt - kvh * P.row_groups;
+            const int64_t piece = (int64_t)w * RTW * 2 + slot;
+            run_int4_segment<D, NG, RTW, C, EXACT>(P, b, kvh, rg * RTW, ctx, blk0 * unit, min(ctx, blk1 * unit),
+                                                   blk1 - blk0 == nb, P.part_o + piece * 16 * D, P.part_ml + piece * 32,
+                                                   lds);
+            slot = 1;
+        }
+        t0 += nb + P.seg_cost;
+        if (t0 >= end) break;
         if (++j == tpb) {
             j = 0;
             do {
                 ++b;
                 ctx = __builtin_amdgcn_readfirstlane(ctx_of(P, b));
-                nb = (ctx + bs - 1) / bs;
+                nb = (ctx + unit - 1) / unit;
             } while (nb == 0 && b + 1 < P.batch);
         }
     }
