@@ -8,7 +8,13 @@
 // consecutive bytes of a page. K's word goes out as it is; V's four bytes are
 // traded within the row's lanes for two 16-bit pieces each (dims 32 apart).
 //
-// Quantisation, whose instructions bound the append. Least and greatest value of
+// The gather is bound by memory, the append by memory and its instructions in
+// turn: 16001 tokens of 8 kv heads of 128 dims, bf16, append 26 us (84 MB, 3.2
+// TB/s; 18.4 with the quantisation left out), gather 21 (4.0). A grid of 2048
+// workgroups that go on to the next rows, their loads ahead, took 28.9 and 25.9,
+// 128 or 512 threads the same as 256. Few tokens: 4.5 and 3.0 us, the latency.
+//
+// Quantisation. Least and greatest value of
 // a group come from 16-bit integers of the floats' order, two to a register, by
 // DPP moves over its G / 8 lanes. The code is round((x - z) / s):
 // (x - z) times the reciprocal of 15 s, kept in 0 .. 1 (the product's clamp), is
@@ -216,21 +222,21 @@ __global__ void __launch_bounds__(kThreads4) kv4_append_kernel(const Kv4Params P
         P.vs[pair] = v_sz;
     }
     uint8_t *const kp = P.kc + at.blk * P.k_bs + h * P.k_hs, *const vp = P.vc + at.blk * P.v_bs + h * P.v_hs;
-    // codes past the caches: 25.1 us against 26.2 (16001 tokens, 8 heads of 128 dims)
-    __builtin_nontemporal_store(k_word, reinterpret_cast<unsigned *>(kp + at.off * (D / 2) + 4 * ((D / 32) * (c & 3) + (c >> 2))));
+    // codes and rows through the caches, for what reads them: stored past them the
+    // gather alone takes 13.9 us (21.4), but with a kernel that reads its rows 39.6
+    // (35.8), and after the append 44 (41); 16001 tokens, 8 heads of 128 dims
+    *reinterpret_cast<unsigned *>(kp + at.off * (D / 2) + 4 * ((D / 32) * (c & 3) + (c >> 2))) = k_word;
     const bool high = c & 4;
     const unsigned u0 = high ? other : v_word, u1 = high ? v_word : other;
     // two pieces, of bytes 0 and 1 or 2 and 3 of u0 and u1: u0's byte, then u1's
     const unsigned both = __builtin_amdgcn_perm(u1, u0, high ? 0x07030602u : 0x05010400u);
     uint8_t *const piece = vp + v_piece<D>(at.off, 4 * (c & 3) + (high ? 2 : 0), c >> 3);
-    __builtin_nontemporal_store((uint16_t)both, reinterpret_cast<uint16_t *>(piece));
-    __builtin_nontemporal_store((uint16_t)(both >> 16), reinterpret_cast<uint16_t *>(piece + D / 8));  // the next l
+    *reinterpret_cast<uint16_t *>(piece) = (uint16_t)both;
+    *reinterpret_cast<uint16_t *>(piece + D / 8) = (uint16_t)(both >> 16);  // the next l
 }
 
 enum { kRowF32 = 0, kRowBf16 = 1, kRowF16 = 2 };
 
-// The rows go past the caches: 13.9 us for 16001 tokens of 8 heads of 128 dims
-// (bf16), 21.5 through them.
 template <int ROW>
 __device__ __forceinline__ void store_row8(void *dst, const int64_t at, const unsigned word, const unsigned sz) {
     const float s = elem_to_float<true>(sz & 0xffffu), z = elem_to_float<true>(sz >> 16);
@@ -239,8 +245,8 @@ __device__ __forceinline__ void store_row8(void *dst, const int64_t at, const un
     for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf((float)((word >> (4 * i)) & 15u), s, z);
     if constexpr (ROW == kRowF32) {
         f32x4_t *const out = reinterpret_cast<f32x4_t *>((float *)dst + at);
-        __builtin_nontemporal_store((f32x4_t){x[0], x[1], x[2], x[3]}, out);
-        __builtin_nontemporal_store((f32x4_t){x[4], x[5], x[6], x[7]}, out + 1);
+        out[0] = (f32x4_t){x[0], x[1], x[2], x[3]};
+        out[1] = (f32x4_t){x[4], x[5], x[6], x[7]};
     } else {
         u32x4_t w;
 #pragma unroll
@@ -252,7 +258,7 @@ __device__ __forceinline__ void store_row8(void *dst, const int64_t at, const un
                 w[i] = (unsigned)__builtin_bit_cast(uint16_t, (_Float16)x[2 * i]) |
                        (unsigned)__builtin_bit_cast(uint16_t, (_Float16)x[2 * i + 1]) << 16;
         }
-        __builtin_nontemporal_store(w, reinterpret_cast<u32x4_t *>((uint16_t *)dst + at));
+        *reinterpret_cast<u32x4_t *>((uint16_t *)dst + at) = w;
     }
 }
 

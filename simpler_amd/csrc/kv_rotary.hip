@@ -13,6 +13,10 @@
 // card, one set where there are few (sets_per_wave). Head dims other than 64,
 // 128 and 256 take a wave per head, elements of a half side by side.
 //
+// Bound by memory, and by its latency and the launch where tokens are few: 9001
+// tokens of 32 + 2 x 8 heads of 128 dims, bf16, 50.9 us (4.5 TB/s of 221 MB;
+// copies reach 5.2); 32 tokens, fp32 with norms, 4.9 us.
+//
 // fp32 arithmetic in the golden's order without fused multiply-adds, as in
 // kv_cache.hip (simpler_setup/goldens/qwen3_14b_decode.py:99-103,207-226).
 
@@ -259,10 +263,11 @@ __global__ void __launch_bounds__(kThreadsR) mrope_kernel(const RotaryParams P) 
                 uint16_t *dst = is_q   ? P.q_out + ((int64_t)t * P.hq + h) * D
                                 : is_k ? P.kc + at.blk * P.k_bs + at.off * P.k_ts + h * P.k_hs
                                        : P.vc + at.blk * P.v_bs + at.off * P.v_ts + h * P.v_hs;
+                // through the caches, for the attention that reads them: past them 47.0 us against
+                // 50.9 (the sizes above), but 71.3 against 68.1 with a kernel that reads q after it
                 const u32x4_t none = {0, 0, 0, 0};
-                __builtin_nontemporal_store(at.ok ? pack8(lo, P.f16) : none, reinterpret_cast<u32x4_t *>(dst + 8 * c));
-                __builtin_nontemporal_store(at.ok ? pack8(hi, P.f16) : none,
-                                            reinterpret_cast<u32x4_t *>(dst + 8 * c + half));
+                *reinterpret_cast<u32x4_t *>(dst + 8 * c) = at.ok ? pack8(lo, P.f16) : none;
+                *reinterpret_cast<u32x4_t *>(dst + 8 * c + half) = at.ok ? pack8(hi, P.f16) : none;
             }
         }
     }
@@ -341,8 +346,10 @@ RotaryFn pick_rotary(const int d, const bool vec) {
 }
 
 // Sets of heads per wave: all of a token's where that still gives the card's
-// 1024 SIMDs kWavesPerSimd waves each, fewer for fewer tokens.
-constexpr int kWavesPerSimd = 4;
+// 1024 SIMDs kWavesPerSimd waves each, fewer for fewer tokens (48 heads of 128
+// dims: 1024 tokens bf16 9.8 us, one set per wave 11.5; 4096 25.3 / 29.0; 2048
+// fp32 18.4 / 22.2; to 512 the same).
+constexpr int kWavesPerSimd = 2;
 int sets_per_wave(const int64_t tokens, const int sets) {
     const int64_t per = tokens * sets / (1024 * kWavesPerSimd);
     return (int)std::min<int64_t>(std::max<int64_t>(per, 1), sets);
