@@ -65,6 +65,9 @@ inline bool is_int4(const SimplerHipPaDecodeArgs *a) {
     return a->kv_format == SIMPLER_HIP_KV_INT4_BF16 || a->kv_format == SIMPLER_HIP_KV_INT4_FP16;
 }
 
+// Tokens per unit of the 4-bit caches' work lists: a chunk of the kernel, or a page.
+inline int int4_unit(const SimplerHipPaDecodeArgs *a) { return std::min(a->block_size, 64); }
+
 int validate(const SimplerHipPaDecodeArgs *a) {
     if (!a) return SIMPLER_HIP_ERR_INVALID;
     if (!a->query || !a->key_cache || !a->value_cache || !a->block_table || !a->context_lens || !a->out)
@@ -113,6 +116,11 @@ int validate(const SimplerHipPaDecodeArgs *a) {
     if ((int64_t)a->batch * a->num_kv_heads * row_tiles * a->max_blocks_per_seq >= (int64_t)1 << 31)
         return SIMPLER_HIP_ERR_UNSUPPORTED;
     if ((int64_t)a->batch * a->num_kv_heads * row_tiles >= (int64_t)1 << 31) return SIMPLER_HIP_ERR_UNSUPPORTED;
+    if (int4) {
+        const int unit = int4_unit(a);
+        const int64_t span = (int64_t)a->max_blocks_per_seq * (a->block_size / unit) + kInt4SegTokens / unit;
+        if ((int64_t)a->batch * a->num_kv_heads * row_tiles * span >= (int64_t)1 << 31) return SIMPLER_HIP_ERR_UNSUPPORTED;
+    }
     return SIMPLER_HIP_OK;
 }
 
@@ -133,9 +141,6 @@ struct Kernels {
     DirectFn direct;
     MergeFn merge;
 };
-
-// Tokens per unit of the work lists: a chunk of the kernel, or a page.
-int int4_unit(const SimplerHipPaDecodeArgs *a) { return std::min(a->block_size, 64); }
 
 KernelPair pick_int4(int d, int groups, int rows, int out) {
     return d == 64    ? pick_int4_d64(groups, rows, out)

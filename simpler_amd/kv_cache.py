@@ -26,7 +26,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .paged_attention import _OUT_DTYPES, PagedAttentionError, _current_stream
+from .paged_attention import _OUT_DTYPES, PagedAttentionError, _current_device, _current_stream
 
 EPS = 1e-6  # the golden's eps (qwen3_14b_decode.py:46)
 
@@ -280,9 +280,6 @@ def _launch(name: str, packed: bytes, device: torch.device, stream: int | None) 
             rc = fn(packed, _current_stream(device) if stream is None else stream)
     if rc != 0:
         raise PagedAttentionError(rc, name)
-
-
-_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 # ---------------------------------------------------------------------------

@@ -127,6 +127,7 @@ def _plain_int4_args(query, key_cache, value_cache, block_table, context_lens, o
     kb, kh, kr, k1 = key_cache.stride()
     vb, vh, vr, v1 = value_cache.stride()
     tb, width = block_table.shape
+    at = query.get_device()
     if not (
         len(qs) in (3, 4) and (qt is torch.bfloat16 or qt is torch.float16) and (ot is torch.float32 or ot is qt)
         and value_cache.dtype is torch.uint8 and v_scale.dtype is torch.float16 and 2 * row == dk
@@ -134,12 +135,17 @@ def _plain_int4_args(query, key_cache, value_cache, block_table, context_lens, o
         and (sn, sh, sb, two) == (nblk, hkv, bs, 2) and dk % groups == 0 and k1 == 1 and v1 == 1 and kr == row
         and vr == row and out.shape == qs and tb == batch and context_lens.shape == (batch,)
         and block_table.dtype is torch.int32 and context_lens.dtype is torch.int32 and query.is_cuda
-        and key_cache.is_cuda and value_cache.is_cuda and k_scale.is_cuda and v_scale.is_cuda and block_table.is_cuda
-        and context_lens.is_cuda and out.is_cuda and query.is_contiguous() and out.is_contiguous()
+        and key_cache.get_device() == at and value_cache.get_device() == at and k_scale.get_device() == at
+        and v_scale.get_device() == at and block_table.get_device() == at and context_lens.get_device() == at
+        and out.get_device() == at and query.is_contiguous() and out.is_contiguous()
         and block_table.is_contiguous() and context_lens.is_contiguous() and k_scale.is_contiguous()
         and v_scale.is_contiguous()
     ):
         return None
+    if hkv == 1:  # strides of dims of one element say nothing
+        kh = vh = 16
+    if nblk == 1:
+        kb = vb = 16
     return _lib.PaDecodeArgs.from_buffer_copy(_ARGS.pack(
         query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(),
         context_lens.data_ptr(), out.data_ptr(), kb, row, kh, vb, row, vh, batch, q_len, hq, hkv, dk, dk, bs, width,
@@ -321,6 +327,9 @@ def _refuse_int4(query, key_cache, value_cache, block_table, context_lens, out, 
         raise ValueError(f"out must have shape {tuple(query.shape)}, got {tuple(out.shape)}")
     if block_table.shape[0] != query.shape[0] or context_lens.shape != query.shape[:1]:
         raise ValueError("block_table/context_lens batch does not match the query")
+    tensors = (query, key_cache, value_cache, block_table, context_lens, out, k_scale, v_scale)
+    if len({t.get_device() for t in tensors}) > 1:
+        raise ValueError("the tensors must be on one device")
     raise ValueError("scale and num_workers must be numbers")
 
 
@@ -335,10 +344,13 @@ def _current_stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def launch(args: _lib.PaDecodeArgs, device: torch.device, stream: int | None = None,
            phases: int = PHASE_MAIN | PHASE_MERGE, key_new: torch.Tensor | None = None,
            value_new: torch.Tensor | None = None, prelude: _lib.DecodePreludeArgs | None = None) -> None:
-    """Enqueue one decode on ``stream`` (default: torch's current stream).
+    """Enqueue one decode on ``stream`` (default: torch's current stream of ``device``), with ``device`` current.
 
     ``phases`` selects the main kernel, the merge kernel or both (the default);
     a merge must follow a main launch with the same args. With ``key_new``
@@ -347,6 +359,9 @@ def launch(args: _lib.PaDecodeArgs, device: torch.device, stream: int | None = N
     ``prelude_args``) after the prelude and append
     (``simpler_hip_pa_decode_prelude``, both phases).
     """
+    if device.index is not None and device.index != _current_device():
+        with torch.cuda.device(device):
+            return launch(args, device, stream, phases, key_new, value_new, prelude)
     lib = _lib.lib()
     if stream is None:
         stream = _current_stream(device)

@@ -321,3 +321,47 @@ def test_captured_graph_replays_with_new_inputs(device):
         graph.replay()
         torch.cuda.synchronize(device)
         assert torch.equal(out.cpu(), want[i])
+
+
+@pytest.mark.parametrize("scale", [-0.05, 0.0, 1e-6, 1.5])
+def test_scales_of_the_scores(scale, device):
+    """Negative, none, next to none and one that makes the softmax pick single tokens."""
+    case = make_int4_case([5, 300, 64], heads=12, kv_heads=2, q_len=2, scale=scale, seed=77)
+    for out in (BF16, FP32):
+        for workers in (0, 5):
+            check(case, device, out, num_workers=workers)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("heads", [3, 7, 16, 24, 40])
+def test_a_bad_query_row_stays_by_itself(value, heads, device):
+    """A row that is not finite shares its tile (and its lanes) with others, whose results do not change."""
+    case = make_int4_case([200, 1, 90], heads=heads, kv_heads=1, seed=heads)
+    for out in (BF16, FP32):
+        for workers in (0, 3):
+            want = decode(case, device, out, num_workers=workers)
+            kept = case.query.clone()
+            case.query[0, 1] = value
+            got = decode(case, device, out, num_workers=workers)
+            case.query = kept
+            assert torch.isnan(got[0, 1]).all()
+            got[0, 1] = want[0, 1]
+            assert torch.equal(got, want)
+
+
+def test_one_page_and_one_head_of_any_stride(device):
+    """Strides of dims of one element say nothing: any are taken."""
+    case = make_int4_case([60], heads=4, kv_heads=1, block=64, extra_width=0, pool_extra=0, seed=3)
+    want = check(case, device)
+    args, opts = case.device_args(device)
+    for i in (1, 2):
+        args[i] = args[i].as_strided(args[i].shape, (0, 1, args[i].stride(2), 1))
+    out = pa.paged_attention_decode(*args, out_dtype=FP32, **opts)
+    assert torch.equal(out.cpu(), want)
+
+
+def test_lengths_and_rows_of_one_work_list(device):
+    """Every number of workers from one to more than there are chunks, over tiles that end inside their slices."""
+    case = make_int4_case([129, 0, 1, 640, 64, 300], heads=6, kv_heads=2, dim=64, group=32, block=128, seed=21)
+    for workers in range(1, 40):
+        check(case, device, FP32, num_workers=workers)

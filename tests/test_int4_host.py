@@ -52,6 +52,7 @@ def decode_args(**kw) -> _lib.PaDecodeArgs:
     (-2, dict(head_dim_k=256, head_dim_v=256, k_token_stride=128, v_token_stride=128, kv_group=32)),  # eight groups
     (-2, dict(head_dim_k=64, head_dim_v=64, k_token_stride=32, v_token_stride=32, kv_group=16)),
     (-1, dict(kv_format=5)), (-1, dict(num_workers=-1)), (-2, dict(max_blocks_per_seq=1 << 25)),
+    (-2, dict(max_blocks_per_seq=(1 << 23) - 2)),  # with what each tile's start is charged, past the lists' 32 bits
 ])
 def test_decode_refusals(want, kw):
     lib = _lib.lib()
@@ -69,7 +70,8 @@ def test_decode_plans(dim, groups):
                 for heads, q_len in ((8, 1), (32, 1), (32, 8), (128, 8)):
                     a = decode_args(head_dim_k=dim, head_dim_v=dim, k_token_stride=dim // 2, v_token_stride=dim // 2,
                                     kv_group=group, block_size=block, kv_format=fmt, out_dtype=out, num_heads=heads,
-                                    q_len=q_len, k_head_stride=block * dim // 2, v_head_stride=block * dim // 2)
+                                    q_len=q_len, k_head_stride=block * dim // 2, v_head_stride=block * dim // 2,
+                                    max_blocks_per_seq=8192 // block)
                     assert pa.kernel_name(a) == "pa_int4_kernel" and pa.plan(a) > 0
                     need = lib.simpler_hip_pa_decode_workspace_size(ctypes.byref(a))
                     assert 256 < need <= 136 << 20  # the fixed scratch of the no-alloc entry
@@ -78,6 +80,14 @@ def test_decode_plans(dim, groups):
                     assert pa.kernel_name(a) == "pa_int4_direct_kernel"
                     a.num_workers = 5
                     assert pa.kernel_name(a) == "pa_int4_kernel" and pa.plan(a) == 5
+
+
+def test_short_contexts_take_one_launch():
+    """A wave's chunks are at most eight, and at most three more than a list worker's."""
+    for batch, tokens, direct in ((32, 4096, True), (32, 4160, False), (8, 2048, True), (8, 2560, False), (128, 1024, True),
+                                  (128, 1088, False), (1, 1536, True), (1, 2048, False), (5000, 512, True)):
+        name = pa.kernel_name(decode_args(batch=batch, max_blocks_per_seq=tokens // 64))
+        assert name == ("pa_int4_direct_kernel" if direct else "pa_int4_kernel"), (batch, tokens)
 
 
 def test_append_and_prelude_entries():
@@ -115,6 +125,26 @@ def test_make_args_packs_four_bit_pools():
     a = pa.make_args(**int4_tensors(key_cache=both[:, 0], value_cache=both[:, 1]))
     assert (a.k_block_stride, a.v_head_stride, a.kv_format) == (2 * 2 * 32 * 64, 32 * 64, pa.KV_INT4_BF16)
     assert a.value_cache - a.key_cache == 2 * 32 * 64
+
+
+def test_make_args_takes_any_stride_of_one_page_and_head():
+    t = int4_tensors(hkv=1, n=1)
+    for name in ("key_cache", "value_cache"):
+        t[name] = t[name].as_strided(t[name].shape, (0, 3, t[name].stride(2), 1))
+    a = pa.make_args(**t)
+    assert (a.k_block_stride, a.k_head_stride, a.v_block_stride, a.v_head_stride) == (16, 16, 16, 16)
+
+
+class Elsewhere(OnDevice):
+    def get_device(self):
+        return 1
+
+
+def test_make_args_refuses_tensors_of_two_devices():
+    t = int4_tensors()
+    for name in ("key_cache", "value_cache", "k_scale", "v_scale", "block_table", "context_lens", "out"):
+        with pytest.raises(ValueError):
+            pa.make_args(**(t | {name: t[name].as_subclass(Elsewhere)}))
 
 
 @pytest.mark.parametrize("kw", [
