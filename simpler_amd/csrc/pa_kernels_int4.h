@@ -39,6 +39,22 @@
 // k-steps are another tile's, so the C copies of a row add up to it at the end.
 // Scales: lane i loads token i's, the wave shares them through LDS.
 // K(i+1) is loaded into K(i)'s registers right after QK(i), V(i+1) after PV(i).
+//
+// What bounds it, measured (8 kv heads of 128 dims unless said; one call with its
+// merge, which takes 5 to 8 us of it; GB/s of all the bytes it has to move):
+// - Up to 8 rows: HBM. 32 sequences of 1024 to 8192 tokens, 4 rows, G = 64: 42.5 us,
+//   4310 GB/s; the main kernel 36.5 us (5020), its loads without the arithmetic 34.9.
+//   8 of 32768, 8 rows, G = 128: 57.5 us, 4970 GB/s.
+// - 16 rows and more, or many groups: VALU instructions, on codes, scales and softmax
+//   of 64 tokens x 16 rows about 800 per chunk (G = 32), half of the SIMD's issue
+//   slots over the kernel and 70% while both its waves run. 13 sequences of 700 to
+//   9000, 32 rows, G = 32, fp16: 50.3 us, 1760 GB/s. With fp32 output the splits
+//   add to them: 37 of 300 to 5000, 4 kv heads of 64 dims, 7 rows: 23.2 us, 1350 GB/s.
+// - Short contexts: latency, about 2.1 us per chunk of a wave after 6 us
+//   (int4_direct_waves in pa_decode.hip).
+// Tried without gain: three waves per SIMD by fewer registers, a scheduling
+// barrier between the tiles, pages loaded through the caches (2 to 5% slower), the
+// row tiles of a kv head as waves of a workgroup (their K and V come from L2).
 #pragma once
 
 #include "pa_kernels_direct.h"
