@@ -26,7 +26,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .paged_attention import _OUT_DTYPES, PagedAttentionError, _current_device, _current_stream
+from .paged_attention import _OUT_DTYPES, PagedAttentionError, _current_device, _current_stream, _raw_stream
 
 EPS = 1e-6  # the golden's eps (qwen3_14b_decode.py:46)
 
@@ -268,16 +268,17 @@ def prelude_args(q_proj: torch.Tensor, k_proj: torch.Tensor, v_proj: torch.Tenso
     return a
 
 
-def _launch(name: str, packed: bytes, device: torch.device, stream: int | None) -> None:
-    """Run the C entry ``name`` on packed args and ``stream`` (default: torch's current one of ``device``), with
+def _launch(name: str, packed: bytes, at: int, stream: int | None) -> None:
+    """Run the C entry ``name`` on packed args and ``stream`` (default: torch's current one of device ``at``), with
     that device current."""
     fn = getattr(_lib.lib(), name)
-    at = device.index
-    if at is None or at == _current_device():
-        rc = fn(packed, _current_stream(device) if stream is None else stream)
+    if stream is None:
+        stream = _current_stream(torch.device("cuda", at)) if _raw_stream is None else _raw_stream(at)
+    if at == _current_device():
+        rc = fn(packed, stream)
     else:
-        with torch.cuda.device(device):
-            rc = fn(packed, _current_stream(device) if stream is None else stream)
+        with torch.cuda.device(at):
+            rc = fn(packed, stream)
     if rc != 0:
         raise PagedAttentionError(rc, name)
 
@@ -409,7 +410,7 @@ def kv4_append(key: torch.Tensor, value: torch.Tensor, slot_mapping: torch.Tenso
     range saturate, and a group with a NaN or an infinity reads back as NaN.
     """
     a = _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, _HALVES)
-    _launch("simpler_hip_kv4_append", a, key.device, stream)
+    _launch("simpler_hip_kv4_append", a, key.get_device(), stream)
 
 
 def kv4_gather(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -427,7 +428,7 @@ def kv4_gather(slot_mapping: torch.Tensor, key_cache: torch.Tensor, value_cache:
                            device=key_cache.device).unbind()
         key, value = (rows[0] if key is None else key), (rows[1] if value is None else value)
     a = _kv4_args(key, value, slot_mapping, key_cache, value_cache, k_scale, v_scale, error_count, _ROWS)
-    _launch("simpler_hip_kv4_gather", a, key.device, stream)
+    _launch("simpler_hip_kv4_gather", a, key.get_device(), stream)
     return key, value
 
 
@@ -506,7 +507,7 @@ def qk_norm_mrope_append(q_proj: torch.Tensor, k_proj: torch.Tensor, v_proj: tor
         num_heads * dim if one else qs[0], hkv * dim if one else ks[0], hkv * dim if one else vs[0],
         kst[0], kst[1], kst[2], vst[0], vst[1], vst[2], tokens, num_heads, hkv, dim, bs, nblk, rope[0],
         _OUT_DTYPES[proj], _OUT_DTYPES[dtype], axes, 1 if interleaved else 0, *sections, *_NO_SECTIONS[axes:], eps)
-    _launch("simpler_hip_qk_norm_mrope_append", packed, q_proj.device, stream)
+    _launch("simpler_hip_qk_norm_mrope_append", packed, at, stream)
     return q_out
 
 
@@ -624,7 +625,7 @@ def release_blocks(ended: torch.Tensor, context_lens: torch.Tensor, block_table:
     count_out, lens_out = torch.empty(batch + 1, dtype=torch.int32, device=device).split_with_sizes((1, batch))
     at = count_out.data_ptr()
     _launch("simpler_hip_release_blocks", _RELEASE.pack(*inputs, at + 4, at, errors, batch, width, block_size,
-                                                        free_blocks.shape[0]), device, stream)
+                                                        free_blocks.shape[0]), device.index, stream)
     return ReleasedBlocks(lens_out, count_out)
 
 
@@ -656,5 +657,5 @@ def assign_slots(new_lens: torch.Tensor, context_lens: torch.Tensor, block_table
     after = at + 3 * n4
     _launch("simpler_hip_assign_slots", _ASSIGN.pack(
         *inputs, at, at + n4, at + 2 * n4, after, after + b4 + 4, after + 2 * b4 + 4, after + 3 * b4 + 4, errors, batch,
-        width, block_size, free_blocks.shape[0], n, 0), device, stream)
+        width, block_size, free_blocks.shape[0], n, 0), device.index, stream)
     return StepSlots(*parts)
