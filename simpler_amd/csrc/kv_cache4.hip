@@ -205,9 +205,9 @@ __global__ void __launch_bounds__(kThreads4) kv4_append_kernel(const Kv4Params P
     const Share<D> me(P.hkv);
     const int c = me.c, h = me.h;
     const int64_t row = min(me.t, P.tokens - 1);
-    const u32x4_t k_raw = *reinterpret_cast<const u32x4_t *>((const uint16_t *)P.key + row * P.key_ts + h * P.key_hs + 8 * c);
-    const u32x4_t v_raw =
-        *reinterpret_cast<const u32x4_t *>((const uint16_t *)P.value + row * P.val_ts + h * P.val_hs + 8 * c);
+    const uint16_t *const kr = (const uint16_t *)P.key + row * P.key_ts + h * P.key_hs + 8 * c;
+    const uint16_t *const vr = (const uint16_t *)P.value + row * P.val_ts + h * P.val_hs + 8 * c;
+    const u32x4_t k_raw = *reinterpret_cast<const u32x4_t *>(kr), v_raw = *reinterpret_cast<const u32x4_t *>(vr);
     const Cell at = cell_of(P, me.t, c == 0 && h == 0);
     unsigned k_word, k_sz, v_word, v_sz;
     quantise8<G / 8, F16>(k_raw, k_word, k_sz);
@@ -277,7 +277,8 @@ __global__ void __launch_bounds__(kThreads4) kv4_gather_kernel(const Kv4Params P
         const uint8_t *const kp = P.kc + at.blk * P.k_bs + h * P.k_hs, *const vp = P.vc + at.blk * P.v_bs + h * P.v_hs;
         k_word = *reinterpret_cast<const unsigned *>(kp + at.off * (D / 2) + 4 * ((D / 32) * (c & 3) + (c >> 2)));
         const uint8_t *const piece = vp + v_piece<D>(at.off, 4 * (c & 3) + (c & 4 ? 2 : 0), c >> 3);
-        both = *reinterpret_cast<const uint16_t *>(piece) | (unsigned)*reinterpret_cast<const uint16_t *>(piece + D / 8) << 16;
+        both = *reinterpret_cast<const uint16_t *>(piece) |
+               (unsigned)*reinterpret_cast<const uint16_t *>(piece + D / 8) << 16;
     }
     // V: the append's trade, back: two pieces hold two bytes of this lane's word and two of the lane 4 away
     const unsigned other = __shfl_xor(both, 4, 64);

@@ -160,8 +160,9 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
             rowlim[r] = min(seg_end, P.causal ? ctx - (P.q_len - 1 - i) : ctx);
         }
     }
+    const int32_t *const table_row = P.block_table + (int64_t)b * (P.max_blocks * P.block_size >> sh);
     const __attribute__((address_space(4))) int32_t *bt_row =
-        (const __attribute__((address_space(4))) int32_t *)(P.block_table + (int64_t)b * (P.max_blocks * P.block_size >> sh));
+        (const __attribute__((address_space(4))) int32_t *)table_row;
     const char *k_head = reinterpret_cast<const char *>(P.k) + (int64_t)kvh * P.k_head_stride;
     const char *v_head = reinterpret_cast<const char *>(P.v) + (int64_t)kvh * P.v_head_stride;
     const unsigned *k_sc = reinterpret_cast<const unsigned *>(P.k_scale);
@@ -248,8 +249,10 @@ __device__ __forceinline__ void run_int4_segment(const KernelParams &P, const in
 #pragma unroll
             for (int j = 0; j < KS; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    f[j][2 * i] = __uint_as_float(raw[r][j][i] << 16), f[j][2 * i + 1] = __uint_as_float(raw[r][j][i] & 0xffff0000u);
+                for (int i = 0; i < 4; ++i) {
+                    f[j][2 * i] = __uint_as_float(raw[r][j][i] << 16);
+                    f[j][2 * i + 1] = __uint_as_float(raw[r][j][i] & 0xffff0000u);
+                }
         }
 #pragma unroll
         for (int j = 0; j < KS; ++j)

@@ -9,9 +9,10 @@
 // keeps them in LDS, instead of a scan launch and an expansion that waits for
 // it. The tokens, the blocks and the requests are shared out among the
 // workgroups; a token finds its request by binary search in the sums. Measured:
-// 256 requests of a token each 2.8 us (release) and 7.7 us (assign), 1024
-// requests with 60 prompts of up to 8000 tokens 4.2 and 10.8; the scans by DPP
-// moves on 32 bits, where 64-bit ones through LDS took 4.5 and 11.7 in the mean.
+// 256 requests of a token each 2.7 us (release) and 4.7 us (assign), 1024
+// requests with 60 prompts of up to 8000 tokens 4.1 and 8.7. Four tokens per
+// thread, one search for them, took 7.7 and 10.8 (their table entries are read
+// one after the other); 64-bit scans through LDS 1.2 and 2.4 us more.
 
 #include <hip/hip_runtime.h>
 
@@ -26,7 +27,6 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
-constexpr int kTokensPerThread = 4;  // consecutive ones: one search for them
 
 // a + b, at most 2^32 - 1: sums that pass it (lengths that no step has) stay there.
 __device__ __forceinline__ unsigned sat_add(const unsigned a, const unsigned b) {
@@ -178,16 +178,6 @@ __global__ void __launch_bounds__(kThreads) assign_kernel(const AssignParams P) 
             }
         }
     }
-    if (lead) {
-        unsigned all_taken, all_refused;
-        (void)block_scan(taken, sums, &all_taken);
-        (void)block_scan(refused, sums, &all_refused);
-        if (threadIdx.x == 0) {
-            P.starts[0] = 0;
-            P.count_out[0] = count - (int)all_taken;
-            if (all_refused && P.err) atomicAdd(P.err, (int)all_refused);
-        }
-    }
     __syncthreads();
 
     struct Request {
@@ -214,35 +204,33 @@ __global__ void __launch_bounds__(kThreads) assign_kernel(const AssignParams P) 
 
     // the tokens
     const int used = saturate(tok_carry);
-    for (int64_t t0 = (int64_t)thread * kTokensPerThread; t0 < P.tokens; t0 += (int64_t)threads * kTokensPerThread) {
-        int b = first_above(ends, P.batch, (int)t0);
-        Request r{};
-        int start = 0;
-        if (b < P.batch) {
-            r = request(b);
-            start = b ? ends[b - 1] : 0;
-        }
-#pragma unroll
-        for (int k = 0; k < kTokensPerThread; ++k) {
-            if (t0 + k >= P.tokens) break;
-            const int t = (int)t0 + k;
-            if (t < used && t >= ends[b]) {
-                b = first_above(ends, P.batch, t);
-                r = request(b);
-                start = ends[b - 1];  // t >= ends[b - 1] of the request before
-            }
-            int slot = -1, pos = -1, req = -1;
-            if (t < used && r.ok) {
-                pos = r.len + (t - start);
+    for (int64_t i = thread; i < P.tokens; i += threads) {
+        const int t = (int)i;
+        int slot = -1, pos = -1, req = -1;
+        if (t < used) {
+            const int b = first_above(ends, P.batch, t);
+            const Request r = request(b);
+            if (r.ok) {
+                pos = r.len + t - (b ? ends[b - 1] : 0);
                 req = b;
                 const int blk = (int)((unsigned)pos / (unsigned)P.bs);
                 const int phys = blk < r.had ? P.table[(int64_t)b * P.width + blk]
                                              : P.free_blocks[count - 1 - (r.first + blk - r.had)];
                 slot = phys < 0 ? -1 : (int)min((int64_t)phys * P.bs + (pos - blk * P.bs), (int64_t)0x7fffffff);
             }
-            P.slots[t] = slot;
-            P.positions[t] = pos;
-            P.requests[t] = req;
+        }
+        P.slots[t] = slot;
+        P.positions[t] = pos;
+        P.requests[t] = req;
+    }
+    if (lead) {
+        unsigned all_taken, all_refused;
+        (void)block_scan(taken, sums, &all_taken);
+        (void)block_scan(refused, sums, &all_refused);
+        if (threadIdx.x == 0) {
+            P.starts[0] = 0;
+            P.count_out[0] = count - (int)all_taken;
+            if (all_refused && P.err) atomicAdd(P.err, (int)all_refused);
         }
     }
 }
@@ -266,7 +254,8 @@ extern "C" int simpler_hip_release_blocks(const SimplerHipReleaseBlocksArgs *a, 
     if (!a->free_count || !a->free_count_out || (a->capacity > 0 && !a->free_blocks) ||
         (a->batch > 0 && (!a->ended || !a->context_lens || !a->block_table || !a->context_lens_out)))
         return SIMPLER_HIP_ERR_INVALID;
-    if ((a->batch > 0 && a->context_lens_out == a->context_lens) || a->free_count_out == a->free_count) return SIMPLER_HIP_ERR_INVALID;
+    if ((a->batch > 0 && a->context_lens_out == a->context_lens) || a->free_count_out == a->free_count)
+        return SIMPLER_HIP_ERR_INVALID;
     if (a->batch > SIMPLER_HIP_STEP_MAX_BATCH) return SIMPLER_HIP_ERR_UNSUPPORTED;
     ReleaseParams P{a->ended,           a->context_lens,   a->block_table, a->free_count,         a->free_blocks,
                     a->context_lens_out, a->free_count_out, a->error_count, a->batch, a->max_blocks_per_seq,
@@ -292,8 +281,7 @@ extern "C" int simpler_hip_assign_slots(const SimplerHipAssignSlotsArgs *a, void
                    a->slot_mapping, a->positions, a->requests,         a->starts,     a->context_lens_out,
                    a->granted,   a->free_count_out, a->error_count,    a->batch,      a->max_blocks_per_seq,
                    a->block_size, a->capacity,    a->num_tokens};
-    const unsigned grid = grid_for(std::max<int64_t>(((int64_t)a->num_tokens + kTokensPerThread - 1) / kTokensPerThread,
-                                                     a->batch));
+    const unsigned grid = grid_for(std::max(a->num_tokens, a->batch));
     hipLaunchKernelGGL(assign_kernel, dim3(grid), dim3(kThreads), (size_t)std::max(a->batch, 1) * 12,
                        (hipStream_t)stream, P);
     return hipGetLastError() == hipSuccess ? SIMPLER_HIP_OK : SIMPLER_HIP_ERR_LAUNCH;

@@ -365,3 +365,24 @@ def test_lengths_and_rows_of_one_work_list(device):
     case = make_int4_case([129, 0, 1, 640, 64, 300], heads=6, kv_heads=2, dim=64, group=32, block=128, seed=21)
     for workers in range(1, 40):
         check(case, device, FP32, num_workers=workers)
+
+
+def test_pages_past_four_gigabytes(device):
+    """Blocks at the end of a pool whose byte offsets pass 32 bits, as the same blocks of a small pool."""
+    blocks, heads, bs, dim, group = 70000, 8, 128, 128, 64  # 4.6 GB of K, as much of V
+    large = kv_cache.alloc_kv4_pools(blocks, bs, heads, dim, group, device=device)
+    small = kv_cache.alloc_kv4_pools(4, bs, heads, dim, group, device=device)
+    gen = torch.Generator(device).manual_seed(1)
+    rows = torch.randn((2, 400, heads, dim), generator=gen, device=device, dtype=BF16)
+    slots = torch.arange(400, device=device, dtype=torch.int32)
+    kv_cache.kv4_append(rows[0], rows[1], slots, *small)
+    kv_cache.kv4_append(rows[0], rows[1], slots + (blocks - 4) * bs, *large)
+    query = torch.randn((2, 32, dim), generator=gen, device=device, dtype=BF16)
+    table = torch.tensor([[0, 1, 2, 3], [3, 2, 1, 0]], dtype=torch.int32, device=device)
+    lens = torch.tensor([400, 10], dtype=torch.int32, device=device)
+    for workers in (0, 7):
+        want, got = (pa.paged_attention_decode(query, p.key_cache, p.value_cache, t, lens, k_scale=p.k_scale,
+                                               v_scale=p.v_scale, num_workers=workers)
+                     for p, t in ((small, table), (large, table + (blocks - 4))))
+        assert torch.equal(got, want)
+        pa.check_errors(device)
