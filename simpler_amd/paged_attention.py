@@ -359,12 +359,13 @@ def launch(args: _lib.PaDecodeArgs, device: torch.device, stream: int | None = N
     ``prelude_args``) after the prelude and append
     (``simpler_hip_pa_decode_prelude``, both phases).
     """
-    if device.index is not None and device.index != _current_device():
+    at = device.index
+    if at is not None and at != _current_device():
         with torch.cuda.device(device):
             return launch(args, device, stream, phases, key_new, value_new, prelude)
     lib = _lib.lib()
     if stream is None:
-        stream = _current_stream(device)
+        stream = _current_stream(device) if at is None or _raw_stream is None else _raw_stream(at)
     both = phases == PHASE_MAIN | PHASE_MERGE
     if prelude is not None:
         what = "simpler_hip_pa_decode_prelude"
@@ -385,10 +386,10 @@ def launch(args: _lib.PaDecodeArgs, device: torch.device, stream: int | None = N
             if both:
                 return lib.simpler_hip_pa_decode(ctypes.byref(args), ws, nbytes, stream)
             return lib.simpler_hip_pa_decode_phase(ctypes.byref(args), ws, nbytes, stream, phases)
-    if both and device.index is not None:
+    if both and at is not None:
         # The stream's buffer is nearly always large enough, and the call itself
         # says if not. Whatever else it refuses is left to the checks below.
-        ws_ptr, ws_bytes = _WORKSPACE.peek(device.index, stream or 0)
+        ws_ptr, ws_bytes = _WORKSPACE.peek(at, stream or 0)
         if ws_ptr:
             rc = call(ws_ptr, ws_bytes)
             if rc == 0:
@@ -464,10 +465,11 @@ def paged_attention_decode(
     if out is None:
         dv = query.shape[-1] if is_int4(key_cache, k_scale) else value_cache.shape[-1]
         out = torch.empty((*query.shape[:-1], dv), dtype=out_dtype, device=query.device)
-    args = make_args(
-        query, key_cache, value_cache, block_table, context_lens, out, scale,
-        causal=causal, num_workers=num_workers, k_scale=k_scale, v_scale=v_scale,
-    )
+    args = _plain_args(query, key_cache, value_cache, block_table, context_lens, out, scale, causal, num_workers,
+                       k_scale, v_scale)
+    if args is None:
+        args = make_args(query, key_cache, value_cache, block_table, context_lens, out, scale, causal=causal,
+                         num_workers=num_workers, k_scale=k_scale, v_scale=v_scale)
     launch(args, query.device)
     return out
 
