@@ -700,10 +700,22 @@ __global__ void __launch_bounds__((64 * int4_direct_waves<D>())) pa_int4_direct_
 
 // The kernels for `rows` query rows per kv head. Two row tiles per wave: not
 // with 256 dims, whose accumulators alone are 128 registers then.
+// Token tiles side by side for up to four rows: four, two where 128 dims are one
+// group and the output has 16 bits. us per call, 4 / 2 tiles, 32 sequences of 1024
+// to 8192, 8 kv heads, 4 rows: 64 dims, G = 64 32.5 / 34.8, G = 32 and fp32 40.2 / 43.2;
+// 128 dims, G = 32 45.7 / 47.1, G = 64 42.5 / 42.3, G = 128 40.2 / 39.7 and with one row
+// 42.3 / 37.9, with fp32 41.1 / 42.0; 256 dims (16 x 4 kv heads), one row 28.2 / 29.5.
+// (For 5 to 8 rows, 2 tiles / 1: 6 rows of 128 dims 35.7 / 36.6, 7 rows of 64
+// dims, fp32 23.1 / 24.4.)
+template <int D, int NG, bool EXACT>
+constexpr int int4_few() {
+    return D == 128 && NG == 1 && !EXACT ? 2 : 4;
+}
+
 template <int D, int NG, bool EXACT>
 KernelPair int4_set(const int rows) {
     KernelPair k{};
-    k.main = rows <= 4 ? pa_int4_kernel<D, NG, 1, 4, EXACT>
+    k.main = rows <= 4 ? pa_int4_kernel<D, NG, 1, int4_few<D, NG, EXACT>(), EXACT>
              : rows <= 8 ? pa_int4_kernel<D, NG, 1, 2, EXACT> : pa_int4_kernel<D, NG, 1, 1, EXACT>;
     if constexpr (D <= 128) k.main_pair = pa_int4_kernel<D, NG, 2, 1, EXACT>;
     return k;
